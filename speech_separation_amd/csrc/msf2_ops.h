@@ -329,6 +329,27 @@ __device__ __forceinline__ float4 bf16x4_ld(const unsigned short* p) {
                        __builtin_bit_cast(float, h.y << 16), __builtin_bit_cast(float, h.y & 0xffff0000u));
 }
 constexpr int DW16_TS = 32;      // frames per block of the bf16 kernel: 48 row reads per 32 results
+// Input rows R0 .. R1 - 1 of a tile into every result row they reach.  Two halves of the tile's rows, because the
+// compiler gives up unrolling one loop over all 48 (64 multiply-adds a row), and what it leaves rolled indexes acc in memory.
+template <int R0, int R1>
+__device__ __forceinline__ void dw16_rows(const unsigned short* __restrict__ xb, int ldx, int s0, int S, const float4 (&w)[17],
+                                          float4 (&acc)[DW16_TS]) {
+#pragma unroll
+    for (int r = R0; r < R1; ++r) {
+        const int s = s0 + r;
+        const float inb = (s >= 0 && s < S) ? 1.f : 0.f;      // see dwconv17_kernel
+        float4 xv = bf16x4_ld(xb + (long)min(max(s, 0), S - 1) * ldx);
+        xv.x *= inb; xv.y *= inb; xv.z *= inb; xv.w *= inb;
+#pragma unroll
+        for (int k = 0; k < 17; ++k) {
+            const int o = r - k + 8;             // the result row this input row feeds through tap k
+            if (o >= 0 && o < DW16_TS) {
+                acc[o].x += w[k].x * xv.x; acc[o].y += w[k].y * xv.y;
+                acc[o].z += w[k].z * xv.z; acc[o].w += w[k].w * xv.w;
+            }
+        }
+    }
+}
 __global__ __launch_bounds__(128, 2) void dwconv17_bf16_kernel(const unsigned short* __restrict__ x, int ldx,
                                                             const float* __restrict__ dw, unsigned short* __restrict__ y,
                                                             int ldy, int S, int C) {
@@ -343,21 +364,8 @@ __global__ __launch_bounds__(128, 2) void dwconv17_bf16_kernel(const unsigned sh
 #pragma unroll
     for (int o = 0; o < DW16_TS; ++o) acc[o] = make_float4(0.f, 0.f, 0.f, 0.f);
     const unsigned short* xb = x + (long)b * S * ldx + 4 * cq;
-#pragma unroll
-    for (int r = -8; r < DW16_TS + 8; ++r) {
-        const int s = s0 + r;
-        const float inb = (s >= 0 && s < S) ? 1.f : 0.f;      // see dwconv17_kernel
-        float4 xv = bf16x4_ld(xb + (long)min(max(s, 0), S - 1) * ldx);
-        xv.x *= inb; xv.y *= inb; xv.z *= inb; xv.w *= inb;
-#pragma unroll
-        for (int k = 0; k < 17; ++k) {
-            const int o = r - k + 8;             // the result row this input row feeds through tap k
-            if (o >= 0 && o < DW16_TS) {
-                acc[o].x += w[k].x * xv.x; acc[o].y += w[k].y * xv.y;
-                acc[o].z += w[k].z * xv.z; acc[o].w += w[k].w * xv.w;
-            }
-        }
-    }
+    dw16_rows<-8, DW16_TS / 2>(xb, ldx, s0, S, w, acc);
+    dw16_rows<DW16_TS / 2, DW16_TS + 8>(xb, ldx, s0, S, w, acc);
     unsigned short* yb = y + (long)b * S * ldy + 4 * cq;
 #pragma unroll
     for (int o = 0; o < DW16_TS; ++o) {
