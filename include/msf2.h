@@ -328,6 +328,74 @@ size_t msf2_pit_si_snr_ws_bytes(int B, int T);
 int msf2_pit_si_snr_noalloc(const float* est, const float* src, float* si_snr, float* best, int* perm, int B, int T,
                             void* stream);
 
+/* ---- operators of a gated recurrent block, with their gradients ------------
+ * What a user needs to train or stream a block of this kind next to the forward above: a group norm with its
+ * activation, a gated linear recurrence, dropout.  The reference trains its blocks through torch.nn autograd
+ * (GroupNorm and Dropout: mossformer2_block.py:508-566); the recurrence has no counterpart there.
+ *
+ * Activations are [B, S, C] in one of the element types below.  Channels are contiguous; `*_batch` and `*_row` are the
+ * strides of the batch and of a frame in ELEMENTS, so a tensor may be a slice of a wider one (value and gate side by side
+ * as one projection writes them).  No alignment beyond the element's is asked for.  Arithmetic, statistics, states and
+ * sums are fp32 or wider whatever the element type.  Outputs must not overlap inputs, except where stated.
+ * `lengths` (int32 [B] on the device, or null: all S): frames at and past lengths[b] belong to no utterance.  They are not
+ * read into any result, whatever they hold, and outputs are zero there.  Values outside [0, S] count as the nearer end. */
+#define MSF2_TYPE_FP32 0
+#define MSF2_TYPE_BF16 1
+#define MSF2_TYPE_FP16 2
+#define MSF2_ACT_NONE 0
+#define MSF2_ACT_SILU 1
+#define MSF2_ACT_SIGMOID 2
+#define MSF2_ACT_RELU 3
+
+/* y = act(norm(x)), or norm(act(x)) with act_first != 0 (the order of TCNBlock.net, mossformer2_block.py:513-519);
+ * norm: per utterance and group of C / groups neighbouring channels, over the utterance's frames and the group's
+ * channels, biased variance + eps, then gamma[c], beta[c] (null: 1, 0).
+ *   stats [B][groups][2] = (mean, 1 / sqrt(var + eps)) of act_first ? act(x) : x; (0, 0) for an empty utterance.
+ * The backward pass takes the stats of the forward and gives dx, and dgamma, dbeta [C] (either may be null). */
+int msf2_group_norm_act(const void* x, int64_t x_batch, int64_t x_row, const float* gamma, const float* beta,
+                        const int32_t* lengths, void* y, int64_t y_batch, int64_t y_row, float* stats, int B, int S, int C,
+                        int groups, float eps, int act, int act_first, int type, void* ws, size_t ws_bytes, void* stream);
+size_t msf2_group_norm_act_ws_bytes(int B, int S, int C, int groups, int type);
+int msf2_group_norm_act_backward(const void* dy, int64_t dy_batch, int64_t dy_row, const void* x, int64_t x_batch,
+                                 int64_t x_row, const float* gamma, const float* beta, const float* stats,
+                                 const int32_t* lengths, void* dx, int64_t dx_batch, int64_t dx_row, float* dgamma,
+                                 float* dbeta, int B, int S, int C, int groups, int act, int act_first, int type, void* ws,
+                                 size_t ws_bytes, void* stream);
+size_t msf2_group_norm_act_backward_ws_bytes(int B, int S, int C, int groups, int type);
+
+/* h_t = a_t h_{t-1} + (1 - a_t) x_t per channel, a_t = sigmoid(gate_t), over the frames of an utterance in order, or from its
+ * last frame to its first with reverse != 0; h_{-1} = h0 (fp32 [B][C], null: zeros).
+ *   last  fp32 [B][C], may be null or h0 itself: the state after the last frame walked (h0 for an empty utterance).
+ *   saved fp32 [B][ceil(S / MSF2_RECURRENCE_SAVE)][C], null unless the backward pass follows: the state before every
+ *         MSF2_RECURRENCE_SAVE-th frame walked, from which the backward pass computes h again.
+ * Backward: dh, and dlast (fp32 [B][C], null: zeros), the gradient of `last`, give dx, dgate and dh0 (fp32 [B][C], may be null
+ * or dlast itself). */
+#define MSF2_RECURRENCE_SAVE 32
+int msf2_gated_recurrence(const void* x, int64_t x_batch, int64_t x_row, const void* gate, int64_t gate_batch,
+                          int64_t gate_row, const float* h0, const int32_t* lengths, void* h, int64_t h_batch,
+                          int64_t h_row, float* last, float* saved, int B, int S, int C, int reverse, int type, void* ws,
+                          size_t ws_bytes, void* stream);
+size_t msf2_gated_recurrence_ws_bytes(int B, int S, int C, int type);
+int msf2_gated_recurrence_backward(const void* dh, int64_t dh_batch, int64_t dh_row, const void* x, int64_t x_batch,
+                                   int64_t x_row, const void* gate, int64_t gate_batch, int64_t gate_row,
+                                   const float* saved, const float* dlast, const int32_t* lengths, void* dx,
+                                   int64_t dx_batch, int64_t dx_row, void* dgate, int64_t dgate_batch, int64_t dgate_row,
+                                   float* dh0, int B, int S, int C, int reverse, int type, void* ws, size_t ws_bytes,
+                                   void* stream);
+size_t msf2_gated_recurrence_backward_ws_bytes(int B, int S, int C, int type);
+
+/* y = residual + keep x 65536 / (65536 - t), t = round(65536 p); residual may be null.  keep is never stored: element (b, s, c)
+ * is kept where 16 bits of a counter-based generator are >= t.  They are half-word c % 8 (the low half of a word first) of
+ * Philox4x32-10 (Salmon et al., SC 2011) with the counter (block, block >> 32, step, site), block = (b S + s) ceil(C / 8) + c / 8,
+ * and the key (seed, seed >> 32), each taken modulo 2^32.
+ *   rng  int64 [2] on the DEVICE = (seed, step): a captured graph draws new masks when the caller advances the step;
+ *   site tells the dropouts of one step apart.
+ * The gradient of x is the same call on dy without a residual.  x may be MSF2_TYPE_*; residual and y are of y_type, which is
+ * x_type, or MSF2_TYPE_FP32 with a narrower x, or narrower with x fp32.  y may be x or residual themselves. */
+int msf2_dropout(const void* x, int64_t x_batch, int64_t x_row, const void* residual, int64_t r_batch, int64_t r_row, void* y,
+                 int64_t y_batch, int64_t y_row, const int64_t* rng, uint32_t site, double p, int B, int S, int C,
+                 int x_type, int y_type, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

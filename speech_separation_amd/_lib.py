@@ -18,6 +18,9 @@ PREC_FP32 = 0
 PREC_BF16 = 1
 TIMED_TCN_POINTWISE = 0   # msf2_timing_begin_kernel: the two-product contraction of a TCN block
 TIMED_HIDDEN_PROJ = 1     # ... the token-shifted to_hidden | to_qk projection of a FLASH layer
+TYPE_FP32, TYPE_BF16, TYPE_FP16 = 0, 1, 2                        # element types of the block operators
+ACT_NONE, ACT_SILU, ACT_SIGMOID, ACT_RELU = 0, 1, 2, 3
+RECURRENCE_SAVE = 32      # frames between two saved states of the gated recurrence
 REC_TCN = 0      # GatedTCNBlock after each FLASH layer (what the reference revision instantiates)
 REC_FSMN = 1     # Gated_FSMN_Block_Dilated (the upstream architecture's block, present in the reference)
 
@@ -64,6 +67,7 @@ class Taps(C.Structure):
 
 # every symbol include/msf2.h declares: name -> (restype, argtypes)
 _vp, _i, _sz, _f = C.c_void_p, C.c_int, C.c_size_t, C.c_float
+_rows = [C.c_void_p, C.c_int64, C.c_int64]        # a [B, S, C] tensor: address, batch and frame strides in elements
 SYMBOLS = {
     "msf2_strerror": (C.c_char_p, [_i]),
     "msf2_last_hip_error": (_i, []),
@@ -92,6 +96,17 @@ SYMBOLS = {
     "msf2_pit_si_snr_ws_bytes": (_sz, [_i, _i]),
     "msf2_pit_si_snr": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _sz, _vp]),
     "msf2_pit_si_snr_noalloc": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp]),
+    "msf2_group_norm_act": (_i, [*_rows, _vp, _vp, _vp, *_rows, _vp, _i, _i, _i, _i, _f, _i, _i, _i, _vp, _sz, _vp]),
+    "msf2_group_norm_act_ws_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "msf2_group_norm_act_backward": (_i, [*_rows, *_rows, _vp, _vp, _vp, _vp, *_rows, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp,
+                                          _sz, _vp]),
+    "msf2_group_norm_act_backward_ws_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "msf2_gated_recurrence": (_i, [*_rows, *_rows, _vp, _vp, *_rows, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "msf2_gated_recurrence_ws_bytes": (_sz, [_i, _i, _i, _i]),
+    "msf2_gated_recurrence_backward": (_i, [*_rows, *_rows, *_rows, _vp, _vp, _vp, *_rows, *_rows, _vp, _i, _i, _i, _i, _i, _vp,
+                                            _sz, _vp]),
+    "msf2_gated_recurrence_backward_ws_bytes": (_sz, [_i, _i, _i, _i]),
+    "msf2_dropout": (_i, [*_rows, *_rows, *_rows, _vp, C.c_uint32, C.c_double, _i, _i, _i, _i, _i, _vp]),
     "msf2_decoder": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _sz, _vp]),
 }
 

@@ -11,6 +11,7 @@ HEADER = os.path.join(os.path.dirname(HERE), "include", "msf2.h")
 UNITS = {
     "msf2_api.hip": ("msf2_common.h", "msf2_gemm.h", "msf2_gemm_bf16.h", "msf2_gemm_bf16_astat.h", "msf2_attn_fused.h",
                      "msf2_linkv_bf16.h", "msf2_ops.h"),
+    "msf2_blocks.hip": ("msf2_common.h", "msf2_rows.h", "msf2_groupnorm.h", "msf2_recurrence.h", "msf2_dropout.h"),
 }
 # Packed fp32 arithmetic stays off: hipcc makes v_pk_add/mul/fma_f32 of ordinary float code by itself, and some of their
 # forms have given wrong results on this hardware now and then.  (The host pass warns that it does not know the feature.)

@@ -1,0 +1,134 @@
+// C-ABI entry points of the block operators: group norm with an activation, gated recurrence, dropout.  All work is
+// enqueued on the caller's stream; nothing here allocates, synchronises or keeps state.
+#include <algorithm>
+#include <cmath>
+#include "msf2_groupnorm.h"
+#include "msf2_recurrence.h"
+#include "msf2_dropout.h"
+
+using namespace msf2;
+
+static inline bool sizes_ok(int B, int S, int C) { return B >= 1 && S >= 1 && C >= 1 && (long)B * S <= (1l << 46) / C; }
+static inline int wide_grid(long n) { return (int)std::min<long>((n + 255) / 256, 1 << 16); }
+
+extern "C" {
+
+size_t msf2_group_norm_act_ws_bytes(int B, int S, int C, int groups, int type) { return 0; }
+
+int msf2_group_norm_act(const void* x, int64_t x_batch, int64_t x_row, const float* gamma, const float* beta,
+                        const int32_t* lengths, void* y, int64_t y_batch, int64_t y_row, float* stats, int B, int S, int C,
+                        int groups, float eps, int act, int act_first, int type, void* ws, size_t ws_bytes, void* stream) {
+    if (!x || !y || !stats || !sizes_ok(B, S, C) || groups < 1 || C % groups || !(eps >= 0.f)) return MSF2_ERR_ARG;
+    if (ws_bytes < msf2_group_norm_act_ws_bytes(B, S, C, groups, type)) return MSF2_ERR_WORKSPACE;
+    hipStream_t st = (hipStream_t)stream;
+    return by_type(type, [&](auto t) {
+        typedef decltype(t) T;
+        return by_act(act, [&](auto a) {
+            constexpr int A = decltype(a)::value;
+            const Rows<const T> xr = {(const T*)x, x_batch, x_row};
+            const Rows<T> yr = {(T*)y, y_batch, y_row};
+            auto go = [&](auto pre, auto post) {
+                gn_stats_kernel<T, decltype(pre)::value><<<B * groups, 256, 0, st>>>(xr, lengths, stats, S, groups, C / groups, eps);
+                gn_apply_kernel<T, decltype(pre)::value, decltype(post)::value>
+                    <<<wide_grid((long)B * S * C), 256, 0, st>>>(xr, gamma, beta, lengths, stats, yr, B, S, C, groups);
+                return check_launch();
+            };
+            std::integral_constant<int, A> on;
+            std::integral_constant<int, MSF2_ACT_NONE> off;
+            return act_first ? go(on, off) : go(off, on);
+        });
+    });
+}
+
+size_t msf2_group_norm_act_backward_ws_bytes(int B, int S, int C, int groups, int type) {
+    if (!sizes_ok(B, S, C) || groups < 1 || C % groups) return 0;
+    return align_up((size_t)B * groups * 2 * sizeof(float));
+}
+
+int msf2_group_norm_act_backward(const void* dy, int64_t dy_batch, int64_t dy_row, const void* x, int64_t x_batch,
+                                 int64_t x_row, const float* gamma, const float* beta, const float* stats,
+                                 const int32_t* lengths, void* dx, int64_t dx_batch, int64_t dx_row, float* dgamma,
+                                 float* dbeta, int B, int S, int C, int groups, int act, int act_first, int type, void* ws,
+                                 size_t ws_bytes, void* stream) {
+    if (!dy || !x || !stats || !dx || !ws || !sizes_ok(B, S, C) || groups < 1 || C % groups) return MSF2_ERR_ARG;
+    if (ws_bytes < msf2_group_norm_act_backward_ws_bytes(B, S, C, groups, type)) return MSF2_ERR_WORKSPACE;
+    hipStream_t st = (hipStream_t)stream;
+    float* coef = (float*)ws;
+    return by_type(type, [&](auto t) {
+        typedef decltype(t) T;
+        return by_act(act, [&](auto a) {
+            constexpr int A = decltype(a)::value;
+            const Rows<const T> xr = {(const T*)x, x_batch, x_row}, dyr = {(const T*)dy, dy_batch, dy_row};
+            const Rows<T> dxr = {(T*)dx, dx_batch, dx_row};
+            auto go = [&](auto pre, auto post) {
+                constexpr int P = decltype(pre)::value, Q = decltype(post)::value;
+                gn_sums_kernel<T, P, Q><<<B * groups, 256, 0, st>>>(dyr, xr, gamma, beta, stats, lengths, coef, dgamma, dbeta, B, S, C, groups, 0);
+                if (dgamma || dbeta)
+                    gn_sums_kernel<T, P, Q><<<C, 256, 0, st>>>(dyr, xr, gamma, beta, stats, lengths, coef, dgamma, dbeta, B, S, C, groups, 1);
+                gn_dx_kernel<T, P, Q><<<wide_grid((long)B * S * C), 256, 0, st>>>(dyr, xr, gamma, beta, stats, lengths, coef, dxr, B, S, C, groups);
+                return check_launch();
+            };
+            std::integral_constant<int, A> on;
+            std::integral_constant<int, MSF2_ACT_NONE> off;
+            return act_first ? go(on, off) : go(off, on);
+        });
+    });
+}
+
+size_t msf2_gated_recurrence_ws_bytes(int B, int S, int C, int type) { return 0; }
+
+int msf2_gated_recurrence(const void* x, int64_t x_batch, int64_t x_row, const void* gate, int64_t gate_batch,
+                          int64_t gate_row, const float* h0, const int32_t* lengths, void* h, int64_t h_batch,
+                          int64_t h_row, float* last, float* saved, int B, int S, int C, int reverse, int type, void* ws,
+                          size_t ws_bytes, void* stream) {
+    if (!x || !gate || !h || !sizes_ok(B, S, C)) return MSF2_ERR_ARG;
+    if (ws_bytes < msf2_gated_recurrence_ws_bytes(B, S, C, type)) return MSF2_ERR_WORKSPACE;
+    return by_type(type, [&](auto t) {
+        typedef decltype(t) T;
+        rec_forward_kernel<T><<<((long)B * C + 255) / 256, 256, 0, (hipStream_t)stream>>>(
+            {(const T*)x, x_batch, x_row}, {(const T*)gate, gate_batch, gate_row}, h0, lengths, {(T*)h, h_batch, h_row}, last, saved, B, S, C, reverse);
+        return check_launch();
+    });
+}
+
+size_t msf2_gated_recurrence_backward_ws_bytes(int B, int S, int C, int type) { return 0; }
+
+int msf2_gated_recurrence_backward(const void* dh, int64_t dh_batch, int64_t dh_row, const void* x, int64_t x_batch,
+                                   int64_t x_row, const void* gate, int64_t gate_batch, int64_t gate_row,
+                                   const float* saved, const float* dlast, const int32_t* lengths, void* dx,
+                                   int64_t dx_batch, int64_t dx_row, void* dgate, int64_t dgate_batch, int64_t dgate_row,
+                                   float* dh0, int B, int S, int C, int reverse, int type, void* ws, size_t ws_bytes,
+                                   void* stream) {
+    if (!dh || !x || !gate || !saved || !dx || !dgate || !sizes_ok(B, S, C)) return MSF2_ERR_ARG;
+    if (ws_bytes < msf2_gated_recurrence_backward_ws_bytes(B, S, C, type)) return MSF2_ERR_WORKSPACE;
+    return by_type(type, [&](auto t) {
+        typedef decltype(t) T;
+        rec_backward_kernel<T><<<((long)B * C + 255) / 256, 256, 0, (hipStream_t)stream>>>(
+            {(const T*)dh, dh_batch, dh_row}, {(const T*)x, x_batch, x_row}, {(const T*)gate, gate_batch, gate_row}, saved, dlast, lengths,
+            {(T*)dx, dx_batch, dx_row}, {(T*)dgate, dgate_batch, dgate_row}, dh0, B, S, C, reverse);
+        return check_launch();
+    });
+}
+
+int msf2_dropout(const void* x, int64_t x_batch, int64_t x_row, const void* residual, int64_t r_batch, int64_t r_row, void* y,
+                 int64_t y_batch, int64_t y_row, const int64_t* rng, uint32_t site, double p, int B, int S, int C,
+                 int x_type, int y_type, void* stream) {
+    if (!x || !y || !rng || !sizes_ok(B, S, C) || !(p >= 0. && p <= 1.)) return MSF2_ERR_ARG;
+    if (x_type != y_type && x_type != MSF2_TYPE_FP32 && y_type != MSF2_TYPE_FP32) return MSF2_ERR_ARG;
+    const unsigned thr = (unsigned)std::floor(p * 65536. + 0.5);
+    const float scale = thr < 65536u ? (float)(65536. / (65536. - thr)) : 0.f;
+    return by_type(x_type, [&](auto tx) {
+        return by_type(y_type, [&](auto ty) {
+            typedef decltype(tx) TX;
+            typedef decltype(ty) TY;
+            if constexpr (std::is_same<TX, TY>::value || std::is_same<TX, float>::value || std::is_same<TY, float>::value) {
+                dropout_kernel<TX, TY><<<wide_grid((long)B * S * ((C + 7) / 8)), 256, 0, (hipStream_t)stream>>>(
+                    {(const TX*)x, x_batch, x_row}, {(const TY*)residual, r_batch, r_row}, {(TY*)y, y_batch, y_row}, rng, site, thr, scale, B, S, C);
+                return check_launch();
+            }
+            return MSF2_ERR_ARG;
+        });
+    });
+}
+
+}  // extern "C"

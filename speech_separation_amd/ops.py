@@ -1,8 +1,11 @@
 """Thin torch-tensor wrappers over the single-operator entry points of libmsf2
 (include/msf2.h).  Host plumbing only: shape checks, output / workspace
 allocation from torch's allocator, the current HIP stream.  Every function
-requires CUDA (HIP) fp32 contiguous tensors and raises if the library is
-missing."""
+raises if the library is missing and requires CUDA (HIP) tensors: contiguous
+fp32 ones, except for the block operators at the end (group norm, gated
+recurrence, dropout), which take fp32, bf16 and fp16 and any batch and frame
+strides as long as channels are contiguous.  Those run on the device of their
+operands, whichever device is current, and on its current stream."""
 import torch
 
 from . import _lib
@@ -169,3 +172,231 @@ def gated_fsmn(x, packed):
     _lib.check(lib.msf2_gated_fsmn(x.data_ptr(), C.byref(w), y.data_ptr(), B, S, dim, inner, ws.data_ptr(), ws.numel(),
                                    _stream(x)), "msf2_gated_fsmn")
     return y
+
+
+# ---- operators of a gated recurrent block: group norm with an activation, gated recurrence, dropout ------------------
+# Plain functions: they record nothing for autograd (speech_separation_amd.autograd does) and they may be captured into a
+# HIP graph, workspaces included, which come from torch's allocator for every call.
+_TYPES = {torch.float32: _lib.TYPE_FP32, torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_FP16}
+
+
+def _rows(t, name, like=None, same_type=True):
+    """Address, batch stride and frame stride of a [B, S, C] operand, `like` another one."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 3 and t.dtype in _TYPES):
+        raise ValueError(f"{name}: expected a [B, S, C] fp32, bf16 or fp16 tensor on the GPU")
+    if like is not None and (t.shape != like.shape or t.device != like.device or (same_type and t.dtype != like.dtype)):
+        raise ValueError(f"{name}: expected shape {tuple(like.shape)}, {like.dtype} on {like.device}, "
+                         f"got {tuple(t.shape)}, {t.dtype} on {t.device}")
+    b, s, c = t.stride()
+    if c != 1 and t.shape[2] > 1:
+        raise ValueError(f"{name}: channels must be contiguous (stride 1), got strides {t.stride()}")
+    return t.data_ptr(), b, s
+
+
+def _span(t):
+    """First address and the one past the last of a tensor's elements."""
+    n = sum((k - 1) * st for k, st in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+    return t.data_ptr(), t.data_ptr() + n * t.element_size()
+
+
+def _clash(t, u):
+    """Whether two tensors share memory.  Interleaved ones (two halves of one wider tensor) do not."""
+    (a, b), (c, d) = _span(t), _span(u)
+    if b <= c or d <= a or a == b or c == d:
+        return False
+    if t.dim() == 3 and t.shape == u.shape and t.stride() == u.stride() and t.element_size() == u.element_size():
+        C, row, e = t.shape[2], t.stride(1), t.element_size()
+        if t.shape[0] > 1 and t.stride(0) % max(row, 1):
+            return True
+        return (c - a) % e != 0 or not C <= (c - a) // e % max(row, 1) <= row - C
+    return True
+
+
+def _out_rows(t, name, like, same_type=True, apart=(), same=()):
+    """_rows of an operand that is written: no two of its elements share an address, nor with those of `apart`; `same` may
+    be the very same tensor."""
+    r = _rows(t, name, like, same_type)
+    (B, S, C), (_, b, s) = t.shape, r
+    if t.numel() and not ((S == 1 or s >= C) and (B == 1 or b >= C) and
+                          (B == 1 or S == 1 or b >= (S - 1) * s + C or s >= (B - 1) * b + C)):
+        raise ValueError(f"{name}: rows of the output overlap (strides {t.stride()})")
+    for u in (*apart, *same):
+        if u is not None and _clash(t, u):
+            if any(u is v for v in same) and u.data_ptr() == t.data_ptr() and u.stride() == t.stride() and u.dtype == t.dtype:
+                continue
+            raise ValueError(f"{name}: the output shares memory with another operand")
+    return r
+
+
+def _aside(t, name, shape, device, dtype=torch.float32):
+    """Address of a contiguous side operand (None: null)."""
+    if t is None:
+        return None
+    if not (isinstance(t, torch.Tensor) and t.device == device and t.dtype == dtype and tuple(t.shape) == shape and t.is_contiguous()):
+        raise ValueError(f"{name}: expected a contiguous {dtype} tensor {shape} on {device}")
+    return t.data_ptr()
+
+
+def _call(name, dev, ws_bytes, args):
+    """Run an entry point on `dev`, with a workspace of that many bytes if it takes one, on dev's current stream."""
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _call(name, dev, ws_bytes, args)
+    if ws_bytes is not None:
+        ws = _ws(ws_bytes, dev)
+        args = (*args, ws.data_ptr(), ws.numel())
+    _lib.check(getattr(_lib.load(), name)(*args, torch.cuda.current_stream(dev).cuda_stream), name)
+
+
+def group_norm_act(x, gamma, beta, groups, eps=1e-5, act=_lib.ACT_NONE, act_first=False, lengths=None):
+    """y = act(norm(x)) of x [B, S, C], or norm(act(x)) with act_first: (y, stats [B, groups, 2] = mean and 1/sqrt(var + eps)
+    for the backward pass).  act: _lib.ACT_*.  gamma, beta: fp32 [C] or None; lengths: int32 [B] or None, the frames of each
+    utterance: frames past them count for nothing and are zero in y.  Reference: TCNBlock.net, mossformer2_block.py:513-519."""
+    lib = _lib.load()
+    xr = _rows(x, "x")
+    B, S, C = x.shape
+    if groups < 1 or C % groups or C < 1:
+        raise ValueError(f"groups = {groups} does not divide {C} channels")
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError("eps must be finite and not negative")
+    if act not in (0, 1, 2, 3):
+        raise ValueError(f"unknown activation {act}")
+    dev = x.device
+    side = (_aside(gamma, "gamma", (C,), dev), _aside(beta, "beta", (C,), dev), _aside(lengths, "lengths", (B,), dev, torch.int32))
+    y = torch.empty((B, S, C), dtype=x.dtype, device=dev)
+    if not (B and S):
+        return y, torch.zeros((B, groups, 2), device=dev)
+    stats = torch.empty((B, groups, 2), device=dev)
+    t = _TYPES[x.dtype]
+    _call("msf2_group_norm_act", dev, lib.msf2_group_norm_act_ws_bytes(B, S, C, groups, t),
+          (*xr, *side, y.data_ptr(), S * C, C, stats.data_ptr(), B, S, C, groups, eps, act, int(act_first), t))
+    return y, stats
+
+
+def group_norm_act_backward(dy, x, gamma, beta, stats, groups, act=_lib.ACT_NONE, act_first=False, lengths=None):
+    """(dx, dgamma, dbeta) of group_norm_act for the gradient dy of y; stats as the forward returned them.  dgamma and dbeta
+    are fp32 [C], summed over utterances and frames (None where gamma or beta is)."""
+    lib = _lib.load()
+    xr, dyr = _rows(x, "x"), _rows(dy, "dy", x)
+    B, S, C = x.shape
+    if groups < 1 or C % groups or C < 1:
+        raise ValueError(f"groups = {groups} does not divide {C} channels")
+    if act not in (0, 1, 2, 3):
+        raise ValueError(f"unknown activation {act}")
+    dev = x.device
+    side = (_aside(gamma, "gamma", (C,), dev), _aside(beta, "beta", (C,), dev), _aside(stats, "stats", (B, groups, 2), dev),
+            _aside(lengths, "lengths", (B,), dev, torch.int32))
+    if side[2] is None:
+        raise ValueError("stats: expected what group_norm_act returned")
+    dx = torch.empty((B, S, C), dtype=x.dtype, device=dev)
+    new = torch.empty if B and S else torch.zeros
+    dgamma = None if gamma is None else new((C,), device=dev)
+    dbeta = None if beta is None else new((C,), device=dev)
+    if B and S:
+        t = _TYPES[x.dtype]
+        _call("msf2_group_norm_act_backward", dev, lib.msf2_group_norm_act_backward_ws_bytes(B, S, C, groups, t),
+              (*dyr, *xr, *side, dx.data_ptr(), S * C, C, None if dgamma is None else dgamma.data_ptr(),
+               None if dbeta is None else dbeta.data_ptr(), B, S, C, groups, act, int(act_first), t))
+    return dx, dgamma, dbeta
+
+
+def gated_recurrence(x, gate, h0=None, lengths=None, reverse=False, last=None, save=False):
+    """h_t = a_t h_{t-1} + (1 - a_t) x_t with a = sigmoid(gate), per channel of x, gate [B, S, C], from h0 (fp32 [B, C], None:
+    zeros): (h, last, saved).  last: fp32 [B, C], the state after the last frame, written into `last` if given, which may be h0
+    itself (a stream that keeps one state).  reverse walks from an utterance's last frame to its first.  lengths: int32 [B] or
+    None, as in group_norm_act; an empty utterance hands h0 on.  saved: with save=True the states that
+    gated_recurrence_backward starts from (fp32, one row in _lib.RECURRENCE_SAVE), else None."""
+    lib = _lib.load()
+    xr, gr = _rows(x, "x"), _rows(gate, "gate", x)
+    B, S, C = x.shape
+    if C < 1:
+        raise ValueError("x has no channels")
+    dev = x.device
+    h0p, lp = _aside(h0, "h0", (B, C), dev), _aside(lengths, "lengths", (B,), dev, torch.int32)
+    if last is None:
+        last = torch.empty((B, C), device=dev)
+    lastp = _aside(last, "last", (B, C), dev)
+    h = torch.empty((B, S, C), dtype=x.dtype, device=dev)
+    saved = torch.empty((B, -(-S // _lib.RECURRENCE_SAVE), C), device=dev) if save else None
+    if B and S:
+        t = _TYPES[x.dtype]
+        _call("msf2_gated_recurrence", dev, lib.msf2_gated_recurrence_ws_bytes(B, S, C, t),
+              (*xr, *gr, h0p, lp, h.data_ptr(), S * C, C, lastp, saved.data_ptr() if save else None, B, S, C, int(reverse), t))
+    elif h0 is None:
+        last.zero_()
+    elif last is not h0:
+        last.copy_(h0)
+    return h, last, saved
+
+
+def gated_recurrence_backward(dh, x, gate, saved, dlast=None, lengths=None, reverse=False, out=None):
+    """(dx, dgate, dh0) of gated_recurrence for the gradients dh of h and dlast (fp32 [B, C] or None) of last; saved as the
+    forward returned it with save=True.  out: a pair of tensors to write dx and dgate into, for instance the two halves of the
+    gradient of the projection that x and gate were cut from."""
+    lib = _lib.load()
+    xr, gr, dhr = _rows(x, "x"), _rows(gate, "gate", x), _rows(dh, "dh", x)
+    B, S, C = x.shape
+    if C < 1:
+        raise ValueError("x has no channels")
+    dev = x.device
+    if out is None:
+        dx, dgate = (torch.empty((B, S, C), dtype=x.dtype, device=dev) for _ in range(2))
+        dxr, dgr = (dx.data_ptr(), S * C, C), (dgate.data_ptr(), S * C, C)
+    else:
+        dx, dgate = out
+        dxr = _out_rows(dx, "dx", x, apart=(dh, x, gate, saved, dlast, dgate))
+        dgr = _out_rows(dgate, "dgate", x, apart=(dh, x, gate, saved, dlast))
+    dlp, lp = _aside(dlast, "dlast", (B, C), dev), _aside(lengths, "lengths", (B,), dev, torch.int32)
+    savedp = _aside(saved, "saved", (B, -(-S // _lib.RECURRENCE_SAVE), C), dev)
+    if savedp is None:
+        raise ValueError("saved: expected what gated_recurrence returned with save=True")
+    if not (B and S):
+        return dx, dgate, torch.zeros((B, C), device=dev) if dlast is None else dlast.clone()
+    dh0 = torch.empty((B, C), device=dev)
+    t = _TYPES[x.dtype]
+    _call("msf2_gated_recurrence_backward", dev, lib.msf2_gated_recurrence_backward_ws_bytes(B, S, C, t),
+          (*dhr, *xr, *gr, savedp, dlp, lp, *dxr, *dgr, dh0.data_ptr(), B, S, C, int(reverse), t))
+    return dx, dgate, dh0
+
+
+def _dropout(x, p, rng, site, residual, y, yr=None):
+    xr = _rows(x, "x")
+    B, S, C = x.shape
+    dev = x.device
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"p = {p} is no probability")
+    if not 0 <= site < 1 << 32:
+        raise ValueError("site must be in [0, 2^32)")
+    if y.dtype not in _TYPES or (y.dtype != x.dtype and torch.float32 not in (x.dtype, y.dtype)):
+        raise ValueError(f"no conversion from {x.dtype} to {y.dtype}")
+    rr = (None, 0, 0) if residual is None else _rows(residual, "residual", y)
+    if yr is None:
+        yr = (y.data_ptr(), S * C, C)
+    rngp = _aside(rng, "rng", (2,), dev, torch.int64)
+    if rngp is None:
+        raise ValueError("rng: expected an int64 tensor (seed, step) on the GPU")
+    if B and S and C:
+        _call("msf2_dropout", dev, None, (*xr, *rr, *yr, rngp, site, p, B, S, C, _TYPES[x.dtype], _TYPES[y.dtype]))
+    return y
+
+
+def dropout(x, p, rng, site=0, residual=None, out=None):
+    """residual + x keep / (1 - p) (no residual: x keep / (1 - p)) of x [B, S, C]; residual is of x's type or fp32, and so is the
+    result.  The mask comes from a counter-based generator and is never stored: it depends on rng = (seed, step), an int64
+    tensor on the GPU, on site, which tells the dropouts of one step apart, and on an element's place, not on strides or
+    types (include/msf2.h).  p counts in steps of 2^-16.  Advance rng[1] after a step's backward pass; a captured graph
+    draws new masks when the program does.  out: where to write, x or residual themselves if wanted."""
+    if not all(isinstance(t, torch.Tensor) for t in (x, *(() if residual is None else (residual,)))):
+        raise ValueError("x, residual: expected tensors")
+    if out is not None:
+        _rows(x, "x")
+        return _dropout(x, p, rng, site, residual, out, _out_rows(out, "out", x, same_type=False, apart=(rng,), same=(x, residual)))
+    return _dropout(x, p, rng, site, residual, torch.empty(x.shape, dtype=(x if residual is None else residual).dtype, device=x.device))
+
+
+def dropout_backward(dy, p, rng, site=0, dtype=None):
+    """The gradient of dropout's x (of type `dtype`, None: dy's) for the gradient dy of its result: dy keep / (1 - p), with
+    the forward's p, rng and site.  The residual's gradient is dy itself."""
+    if not isinstance(dy, torch.Tensor):
+        raise ValueError("dy: expected a tensor")
+    return _dropout(dy, p, rng, site, None, torch.empty(dy.shape, dtype=dtype or dy.dtype, device=dy.device))
