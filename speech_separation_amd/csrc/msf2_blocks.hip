@@ -75,23 +75,25 @@ int msf2_group_norm_act_backward(const void* dy, int64_t dy_batch, int64_t dy_ro
     });
 }
 
-size_t msf2_gated_recurrence_ws_bytes(int B, int S, int C, int type) { return 0; }
+size_t msf2_gated_recurrence_ws_bytes(int B, int S, int C, int type) {
+    return sizes_ok(B, S, C) && type >= MSF2_TYPE_FP32 && type <= MSF2_TYPE_FP16 ? rec_ws_bytes(B, S, C, type == MSF2_TYPE_FP32 ? 4 : 2) : 0;
+}
 
 int msf2_gated_recurrence(const void* x, int64_t x_batch, int64_t x_row, const void* gate, int64_t gate_batch,
                           int64_t gate_row, const float* h0, const int32_t* lengths, void* h, int64_t h_batch,
                           int64_t h_row, float* last, float* saved, int B, int S, int C, int reverse, int type, void* ws,
                           size_t ws_bytes, void* stream) {
     if (!x || !gate || !h || !sizes_ok(B, S, C)) return MSF2_ERR_ARG;
-    if (ws_bytes < msf2_gated_recurrence_ws_bytes(B, S, C, type)) return MSF2_ERR_WORKSPACE;
+    const size_t need = msf2_gated_recurrence_ws_bytes(B, S, C, type);
+    if (need && (!ws || ws_bytes < need)) return MSF2_ERR_WORKSPACE;
     return by_type(type, [&](auto t) {
         typedef decltype(t) T;
-        rec_forward_kernel<T><<<((long)B * C + 255) / 256, 256, 0, (hipStream_t)stream>>>(
-            {(const T*)x, x_batch, x_row}, {(const T*)gate, gate_batch, gate_row}, h0, lengths, {(T*)h, h_batch, h_row}, last, saved, B, S, C, reverse);
-        return check_launch();
+        return run_recurrence<T>({(const T*)x, x_batch, x_row}, {(const T*)gate, gate_batch, gate_row}, h0, lengths, {(T*)h, h_batch, h_row},
+                                 last, saved, B, S, C, reverse, ws, (hipStream_t)stream);
     });
 }
 
-size_t msf2_gated_recurrence_backward_ws_bytes(int B, int S, int C, int type) { return 0; }
+size_t msf2_gated_recurrence_backward_ws_bytes(int B, int S, int C, int type) { return msf2_gated_recurrence_ws_bytes(B, S, C, type); }
 
 int msf2_gated_recurrence_backward(const void* dh, int64_t dh_batch, int64_t dh_row, const void* x, int64_t x_batch,
                                    int64_t x_row, const void* gate, int64_t gate_batch, int64_t gate_row,
@@ -100,13 +102,13 @@ int msf2_gated_recurrence_backward(const void* dh, int64_t dh_batch, int64_t dh_
                                    float* dh0, int B, int S, int C, int reverse, int type, void* ws, size_t ws_bytes,
                                    void* stream) {
     if (!dh || !x || !gate || !saved || !dx || !dgate || !sizes_ok(B, S, C)) return MSF2_ERR_ARG;
-    if (ws_bytes < msf2_gated_recurrence_backward_ws_bytes(B, S, C, type)) return MSF2_ERR_WORKSPACE;
+    const size_t need = msf2_gated_recurrence_backward_ws_bytes(B, S, C, type);
+    if (need && (!ws || ws_bytes < need)) return MSF2_ERR_WORKSPACE;
     return by_type(type, [&](auto t) {
         typedef decltype(t) T;
-        rec_backward_kernel<T><<<((long)B * C + 255) / 256, 256, 0, (hipStream_t)stream>>>(
-            {(const T*)dh, dh_batch, dh_row}, {(const T*)x, x_batch, x_row}, {(const T*)gate, gate_batch, gate_row}, saved, dlast, lengths,
-            {(T*)dx, dx_batch, dx_row}, {(T*)dgate, dgate_batch, dgate_row}, dh0, B, S, C, reverse);
-        return check_launch();
+        return run_recurrence_backward<T>({(const T*)dh, dh_batch, dh_row}, {(const T*)x, x_batch, x_row}, {(const T*)gate, gate_batch, gate_row},
+                                          saved, dlast, lengths, {(T*)dx, dx_batch, dx_row}, {(T*)dgate, dgate_batch, dgate_row}, dh0, B, S, C,
+                                          reverse, ws, (hipStream_t)stream);
     });
 }
 
@@ -122,9 +124,8 @@ int msf2_dropout(const void* x, int64_t x_batch, int64_t x_row, const void* resi
             typedef decltype(tx) TX;
             typedef decltype(ty) TY;
             if constexpr (std::is_same<TX, TY>::value || std::is_same<TX, float>::value || std::is_same<TY, float>::value) {
-                dropout_kernel<TX, TY><<<wide_grid((long)B * S * ((C + 7) / 8)), 256, 0, (hipStream_t)stream>>>(
-                    {(const TX*)x, x_batch, x_row}, {(const TY*)residual, r_batch, r_row}, {(TY*)y, y_batch, y_row}, rng, site, thr, scale, B, S, C);
-                return check_launch();
+                return run_dropout<TX, TY>({(const TX*)x, x_batch, x_row}, {(const TY*)residual, r_batch, r_row}, {(TY*)y, y_batch, y_row}, rng, site,
+                                           thr, scale, B, S, C, (hipStream_t)stream);
             }
             return MSF2_ERR_ARG;
         });

@@ -1,5 +1,6 @@
 // Dropout from a counter-based generator, with the residual addition.
 #pragma once
+#include <algorithm>
 #include "msf2_rows.h"
 
 namespace msf2 {
@@ -16,24 +17,75 @@ __device__ __forceinline__ uint4 philox10(uint4 c, uint2 k) {
     return c;
 }
 
-// one thread 8 neighbouring channels of a frame: the 128 bits of one generator call
-template <class TX, class TY>
+// y = residual + x keep scale of `rows` frames (of utterance blockIdx.y where the operands' utterances do not follow one
+// another).  A thread takes U times 8 neighbouring channels of a frame, the 128 bits of one generator call: 16 bits an element, because the
+// generator's 20 wide multiplications (a quarter of the vector rate each) would otherwise bind the kernel before memory does.
+// All loads go out before the first of them.
+template <class TX, class TY, bool RES, int U>
 __global__ __launch_bounds__(256) void dropout_kernel(Rows<const TX> x, Rows<const TY> res, Rows<TY> y, const int64_t* rng,
-                                                      unsigned site, unsigned thr, float scale, int B, int S, int C) {
-    const int per = (C + 7) / 8;
+                                                      unsigned site, unsigned thr, float scale, Divider per, unsigned blocks,
+                                                      long block0, long block_batch, int C) {
     const uint64_t seed = rng[0], step = rng[1];
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < (long)B * S * per; i += (long)gridDim.x * 256) {
-        const int c0 = i % per * 8, s = i / per % S, b = i / per / S;
-        const uint4 r = philox10(make_uint4((unsigned)i, (unsigned)((uint64_t)i >> 32), (unsigned)step, site),
+    const long b = blockIdx.y;
+    const unsigned i0 = blockIdx.x * (256u * U) + threadIdx.x;
+    typename VecOf<TX, 8>::type xv[U];
+    typename VecOf<TY, 8>::type rv[U];
+    unsigned row[U];
+    int c[U], n[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const unsigned i = min(i0 + u * 256u, blocks - 1);
+        row[u] = per.div(i);
+        c[u] = (int)(i - row[u] * per.d) * 8;
+        n[u] = i0 + u * 256u < blocks ? min(C - c[u], 8) : 0;
+        xv[u] = n[u] == 8 ? load_vec<8>(x.at(b, row[u]) + c[u]) : load_some<8>(x.at(b, row[u]) + c[u], n[u]);
+        if constexpr (RES) rv[u] = n[u] == 8 ? load_vec<8>(res.at(b, row[u]) + c[u]) : load_some<8>(res.at(b, row[u]) + c[u], n[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint64_t block = (uint64_t)(block0 + b * block_batch) + i0 + u * 256u;
+        const uint4 r = philox10(make_uint4((unsigned)block, (unsigned)(block >> 32), (unsigned)step, site),
                                  make_uint2((unsigned)seed, (unsigned)(seed >> 32)));
         const unsigned w[4] = {r.x, r.y, r.z, r.w};
-        for (int j = 0; j < 8 && c0 + j < C; ++j) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
             const unsigned bits = j & 1 ? w[j >> 1] >> 16 : w[j >> 1] & 0xFFFF;
-            float v = bits >= thr ? (float)x.at(b, s)[c0 + j] * scale : 0.f;
-            if (res.p) v += (float)res.at(b, s)[c0 + j];
-            y.at(b, s)[c0 + j] = (TY)v;
+            v[j] = bits >= thr ? (float)xv[u][j] * scale : 0.f;
+            if constexpr (RES) v[j] += (float)rv[u][j];
         }
+        if (n[u] == 8) store_vec<8>(y.at(b, row[u]) + c[u], v);
+        else store_some<8>(y.at(b, row[u]) + c[u], n[u], v);
     }
+}
+
+// Utterances that follow one another without a gap are walked as one; a launch takes less than 2^31 generator calls.
+template <class TX, class TY>
+static int run_dropout(Rows<const TX> x, Rows<const TY> res, Rows<TY> y, const int64_t* rng, unsigned site, unsigned thr, float scale,
+                       int B, int S, int C, hipStream_t st) {
+    constexpr int U = 2;
+    long rows = S, batches = B;
+    auto whole = [&](long batch, long row) { return batch == (long)S * row; };
+    if (S == 1) {
+        x.row = x.batch; res.row = res.batch; y.row = y.batch;
+        rows = B; batches = 1;
+    } else if (B > 1 && whole(x.batch, x.row) && whole(y.batch, y.row) && (!res.p || whole(res.batch, res.row))) {
+        rows = (long)B * S; batches = 1;
+    }
+    const long per = (C + 7) / 8, most = ((1l << 31) - 1) / per;
+    const Divider by((unsigned)per);
+    for (long b = 0; b < batches; b += 65535)
+        for (long r = 0; r < rows; r += most) {
+            const unsigned blocks = (unsigned)(std::min(most, rows - r) * per);
+            const dim3 grid((blocks + 256u * U - 1) / (256u * U), (unsigned)std::min(65535l, batches - b));
+            const Rows<const TX> xr = {x.at(b, r), x.batch, x.row};
+            const Rows<const TY> rr = {res.p ? res.at(b, r) : nullptr, res.batch, res.row};
+            const Rows<TY> yr = {y.at(b, r), y.batch, y.row};
+            const long block0 = (b * rows + r) * per;
+            if (res.p) dropout_kernel<TX, TY, true, U><<<grid, 256, 0, st>>>(xr, rr, yr, rng, site, thr, scale, by, blocks, block0, rows * per, C);
+            else dropout_kernel<TX, TY, false, U><<<grid, 256, 0, st>>>(xr, rr, yr, rng, site, thr, scale, by, blocks, block0, rows * per, C);
+        }
+    return check_launch();
 }
 
 }  // namespace msf2

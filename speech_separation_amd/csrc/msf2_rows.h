@@ -25,6 +25,45 @@ template <class T> struct Rows {
     __host__ __device__ T* at(long b, long s) const { return p + b * batch + s * row; }
 };
 
+// V neighbouring elements at any address that suits one element: gfx950 loads and stores 16 bytes at any byte address, so odd
+// widths and slices need no form of their own (an access that straddles two lines costs the second line).
+template <class T, int V> struct VecOf {
+    typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+};
+template <int V, class T> __device__ __forceinline__ typename VecOf<T, V>::type load_vec(const T* p) {
+    return *reinterpret_cast<const typename VecOf<T, V>::type*>(p);
+}
+// the first n < V of them, zeros behind
+template <int V, class T> __device__ __forceinline__ typename VecOf<T, V>::type load_some(const T* p, int n) {
+    typename VecOf<T, V>::type v = {};
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        if (j < n) v[j] = p[j];
+    return v;
+}
+template <int V, class T> __device__ __forceinline__ void store_vec(T* p, const float (&f)[V]) {
+    typename VecOf<T, V>::type v;
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = (T)f[j];
+    *reinterpret_cast<typename VecOf<T, V>::type*>(p) = v;
+}
+template <int V, class T> __device__ __forceinline__ void store_some(T* p, int n, const float (&f)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        if (j < n) p[j] = (T)f[j];
+}
+
+// n / d for n < 2^31 by one multiplication: with 2^(l-1) < d <= 2^l the factor m = 2^(31+l) / d + 1 is off by less than 1, so
+// n m / 2^(31+l) is off by less than 1 / d and its whole part is right.
+struct Divider {
+    unsigned d, m, shift;
+    explicit Divider(unsigned d_) : d(d_), shift(31) {
+        while ((1ull << (shift - 31)) < d) ++shift;
+        m = (unsigned)((1ull << shift) / d + 1);
+    }
+    __device__ __forceinline__ unsigned div(unsigned n) const { return (unsigned)((uint64_t)n * m >> shift); }
+};
+
 // Frames of utterance b: lengths[b] held to [0, S], all S without lengths.
 __device__ __forceinline__ int frames_of(const int* lengths, int b, int S) {
     return lengths ? min(max(lengths[b], 0), S) : S;
