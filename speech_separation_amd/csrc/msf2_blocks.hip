@@ -9,40 +9,38 @@
 using namespace msf2;
 
 static inline bool sizes_ok(int B, int S, int C) { return B >= 1 && S >= 1 && C >= 1 && (long)B * S <= (1l << 46) / C; }
-static inline int wide_grid(long n) { return (int)std::min<long>((n + 255) / 256, 1 << 16); }
+static inline bool type_ok(int type) { return type == MSF2_TYPE_FP32 || type == MSF2_TYPE_BF16 || type == MSF2_TYPE_FP16; }
+static inline int type_bytes(int type) { return type == MSF2_TYPE_FP32 ? 4 : 2; }
+static inline bool norm_ok(int B, int S, int C, int groups, int type) {
+    return sizes_ok(B, S, C) && groups >= 1 && C % groups == 0 && type_ok(type);
+}
 
 extern "C" {
 
-size_t msf2_group_norm_act_ws_bytes(int B, int S, int C, int groups, int type) { return 0; }
+size_t msf2_group_norm_act_ws_bytes(int B, int S, int C, int groups, int type) {
+    return norm_ok(B, S, C, groups, type) ? gn_ws_bytes(B, S, C, groups, type_bytes(type), false) : 0;
+}
 
 int msf2_group_norm_act(const void* x, int64_t x_batch, int64_t x_row, const float* gamma, const float* beta,
                         const int32_t* lengths, void* y, int64_t y_batch, int64_t y_row, float* stats, int B, int S, int C,
                         int groups, float eps, int act, int act_first, int type, void* ws, size_t ws_bytes, void* stream) {
-    if (!x || !y || !stats || !sizes_ok(B, S, C) || groups < 1 || C % groups || !(eps >= 0.f)) return MSF2_ERR_ARG;
+    if (!x || !y || !stats || !ws || !norm_ok(B, S, C, groups, type) || !(eps >= 0.f)) return MSF2_ERR_ARG;
     if (ws_bytes < msf2_group_norm_act_ws_bytes(B, S, C, groups, type)) return MSF2_ERR_WORKSPACE;
-    hipStream_t st = (hipStream_t)stream;
     return by_type(type, [&](auto t) {
         typedef decltype(t) T;
         return by_act(act, [&](auto a) {
-            constexpr int A = decltype(a)::value;
-            const Rows<const T> xr = {(const T*)x, x_batch, x_row};
-            const Rows<T> yr = {(T*)y, y_batch, y_row};
             auto go = [&](auto pre, auto post) {
-                gn_stats_kernel<T, decltype(pre)::value><<<B * groups, 256, 0, st>>>(xr, lengths, stats, S, groups, C / groups, eps);
-                gn_apply_kernel<T, decltype(pre)::value, decltype(post)::value>
-                    <<<wide_grid((long)B * S * C), 256, 0, st>>>(xr, gamma, beta, lengths, stats, yr, B, S, C, groups);
-                return check_launch();
+                return run_group_norm<T, decltype(pre)::value, decltype(post)::value>(
+                    {(const T*)x, x_batch, x_row}, gamma, beta, lengths, {(T*)y, y_batch, y_row}, stats, B, S, C, groups, eps, ws, (hipStream_t)stream);
             };
-            std::integral_constant<int, A> on;
-            std::integral_constant<int, MSF2_ACT_NONE> off;
-            return act_first ? go(on, off) : go(off, on);
+            std::integral_constant<int, MSF2_ACT_NONE> none;
+            return act_first ? go(a, none) : go(none, a);
         });
     });
 }
 
 size_t msf2_group_norm_act_backward_ws_bytes(int B, int S, int C, int groups, int type) {
-    if (!sizes_ok(B, S, C) || groups < 1 || C % groups) return 0;
-    return align_up((size_t)B * groups * 2 * sizeof(float));
+    return norm_ok(B, S, C, groups, type) ? gn_ws_bytes(B, S, C, groups, type_bytes(type), true) : 0;
 }
 
 int msf2_group_norm_act_backward(const void* dy, int64_t dy_batch, int64_t dy_row, const void* x, int64_t x_batch,
@@ -50,33 +48,24 @@ int msf2_group_norm_act_backward(const void* dy, int64_t dy_batch, int64_t dy_ro
                                  const int32_t* lengths, void* dx, int64_t dx_batch, int64_t dx_row, float* dgamma,
                                  float* dbeta, int B, int S, int C, int groups, int act, int act_first, int type, void* ws,
                                  size_t ws_bytes, void* stream) {
-    if (!dy || !x || !stats || !dx || !ws || !sizes_ok(B, S, C) || groups < 1 || C % groups) return MSF2_ERR_ARG;
+    if (!dy || !x || !stats || !dx || !ws || !norm_ok(B, S, C, groups, type)) return MSF2_ERR_ARG;
     if (ws_bytes < msf2_group_norm_act_backward_ws_bytes(B, S, C, groups, type)) return MSF2_ERR_WORKSPACE;
-    hipStream_t st = (hipStream_t)stream;
-    float* coef = (float*)ws;
     return by_type(type, [&](auto t) {
         typedef decltype(t) T;
         return by_act(act, [&](auto a) {
-            constexpr int A = decltype(a)::value;
-            const Rows<const T> xr = {(const T*)x, x_batch, x_row}, dyr = {(const T*)dy, dy_batch, dy_row};
-            const Rows<T> dxr = {(T*)dx, dx_batch, dx_row};
             auto go = [&](auto pre, auto post) {
-                constexpr int P = decltype(pre)::value, Q = decltype(post)::value;
-                gn_sums_kernel<T, P, Q><<<B * groups, 256, 0, st>>>(dyr, xr, gamma, beta, stats, lengths, coef, dgamma, dbeta, B, S, C, groups, 0);
-                if (dgamma || dbeta)
-                    gn_sums_kernel<T, P, Q><<<C, 256, 0, st>>>(dyr, xr, gamma, beta, stats, lengths, coef, dgamma, dbeta, B, S, C, groups, 1);
-                gn_dx_kernel<T, P, Q><<<wide_grid((long)B * S * C), 256, 0, st>>>(dyr, xr, gamma, beta, stats, lengths, coef, dxr, B, S, C, groups);
-                return check_launch();
+                return run_group_norm_backward<T, decltype(pre)::value, decltype(post)::value>(
+                    {(const T*)dy, dy_batch, dy_row}, {(const T*)x, x_batch, x_row}, gamma, beta, stats, lengths, {(T*)dx, dx_batch, dx_row}, dgamma,
+                    dbeta, B, S, C, groups, ws, (hipStream_t)stream);
             };
-            std::integral_constant<int, A> on;
-            std::integral_constant<int, MSF2_ACT_NONE> off;
-            return act_first ? go(on, off) : go(off, on);
+            std::integral_constant<int, MSF2_ACT_NONE> none;
+            return act_first ? go(a, none) : go(none, a);
         });
     });
 }
 
 size_t msf2_gated_recurrence_ws_bytes(int B, int S, int C, int type) {
-    return sizes_ok(B, S, C) && type >= MSF2_TYPE_FP32 && type <= MSF2_TYPE_FP16 ? rec_ws_bytes(B, S, C, type == MSF2_TYPE_FP32 ? 4 : 2) : 0;
+    return sizes_ok(B, S, C) && type_ok(type) ? rec_ws_bytes(B, S, C, type_bytes(type)) : 0;
 }
 
 int msf2_gated_recurrence(const void* x, int64_t x_batch, int64_t x_row, const void* gate, int64_t gate_batch,
