@@ -8,7 +8,8 @@
 
 using namespace msf2;
 
-static inline bool sizes_ok(int B, int S, int C) { return B >= 1 && S >= 1 && C >= 1 && (long)B * S <= (1l << 46) / C; }
+// S below 2^30: frame indices, and the end of the tile that holds the last one, stay below 2^31
+static inline bool sizes_ok(int B, int S, int C) { return B >= 1 && S >= 1 && S < 1 << 30 && C >= 1 && (long)B * S <= (1l << 46) / C; }
 static inline bool type_ok(int type) { return type == MSF2_TYPE_FP32 || type == MSF2_TYPE_BF16 || type == MSF2_TYPE_FP16; }
 static inline int type_bytes(int type) { return type == MSF2_TYPE_FP32 ? 4 : 2; }
 static inline bool norm_ok(int B, int S, int C, int groups, int type) {
@@ -65,7 +66,7 @@ int msf2_group_norm_act_backward(const void* dy, int64_t dy_batch, int64_t dy_ro
 }
 
 size_t msf2_gated_recurrence_ws_bytes(int B, int S, int C, int type) {
-    return sizes_ok(B, S, C) && type_ok(type) ? rec_ws_bytes(B, S, C, type_bytes(type), false) : 0;
+    return sizes_ok(B, S, C) && type_ok(type) ? rec_ws_bytes(B, S, C, type_bytes(type)) : 0;
 }
 
 int msf2_gated_recurrence(const void* x, int64_t x_batch, int64_t x_row, const void* gate, int64_t gate_batch,
@@ -78,12 +79,12 @@ int msf2_gated_recurrence(const void* x, int64_t x_batch, int64_t x_row, const v
     return by_type(type, [&](auto t) {
         typedef decltype(t) T;
         return run_recurrence<T>({(const T*)x, x_batch, x_row}, {(const T*)gate, gate_batch, gate_row}, h0, lengths, {(T*)h, h_batch, h_row},
-                                 last, saved, B, S, C, reverse, ws, (hipStream_t)stream);
+                                 last, saved, B, S, C, reverse != 0, ws, (hipStream_t)stream);
     });
 }
 
 size_t msf2_gated_recurrence_backward_ws_bytes(int B, int S, int C, int type) {
-    return sizes_ok(B, S, C) && type_ok(type) ? rec_ws_bytes(B, S, C, type_bytes(type), true) : 0;
+    return sizes_ok(B, S, C) && type_ok(type) ? rec_ws_bytes(B, S, C, type_bytes(type)) : 0;
 }
 
 int msf2_gated_recurrence_backward(const void* dh, int64_t dh_batch, int64_t dh_row, const void* x, int64_t x_batch,
@@ -99,7 +100,7 @@ int msf2_gated_recurrence_backward(const void* dh, int64_t dh_batch, int64_t dh_
         typedef decltype(t) T;
         return run_recurrence_backward<T>({(const T*)dh, dh_batch, dh_row}, {(const T*)x, x_batch, x_row}, {(const T*)gate, gate_batch, gate_row},
                                           saved, dlast, lengths, {(T*)dx, dx_batch, dx_row}, {(T*)dgate, dgate_batch, dgate_row}, dh0, B, S, C,
-                                          reverse, ws, (hipStream_t)stream);
+                                          reverse != 0, ws, (hipStream_t)stream);
     });
 }
 

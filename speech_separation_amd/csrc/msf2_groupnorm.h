@@ -58,7 +58,7 @@ template <int V, class T> __device__ __forceinline__ typename VecOf<T, V>::type 
     return have >= V ? load_vec<V>(p) : load_some<V>(p, have);
 }
 template <int V, class T> __device__ __forceinline__ void gn_store(T* p, int have, const float (&f)[V]) {
-    if (have >= V) store_vec<V>(p, f);
+    if (have >= V) store_vec<V, true>(p, f);
     else store_some<V>(p, have, f);
 }
 
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(GN_T) void gn_moments_kernel(Rows<const T> x, const
     if (at.have > 0 && s0 + at.r0 < s1) {
         const auto k = gn_load<V>(x.at(at.b, s0 + at.r0) + at.c, at.have);
 #pragma unroll
-        for (int v = 0; v < V; ++v) K[v] = act_f<PRE>((float)k[v]);
+        for (int v = 0; v < V; ++v) K[v] = act_f<PRE, fine<T>()>((float)k[v]);
         for (int r = s0 + at.r0; r < s1; r += U * at.step) {
             typename VecOf<T, V>::type u[U];
 #pragma unroll
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(GN_T) void gn_moments_kernel(Rows<const T> x, const
                 ++count;
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    const float d = act_f<PRE>((float)u[j][v]) - K[v];
+                    const float d = act_f<PRE, fine<T>()>((float)u[j][v]) - K[v];
                     s[v] += d;
                     q[v] = fmaf(d, d, q[v]);
                 }
@@ -201,7 +201,7 @@ __global__ __launch_bounds__(GN_T) void gn_apply_kernel(Rows<const T> x, const f
             float f[V];
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                f[v] = act_f<POST>(fmaf(act_f<PRE>((float)u[j][v]) - mean[v], ga[v], be[v]));
+                f[v] = act_f<POST, fine<T>()>(fmaf(act_f<PRE, fine<T>()>((float)u[j][v]) - mean[v], ga[v], be[v]));
                 if (s >= n) f[v] = 0.f;
             }
             gn_store<V>(y.at(at.b, s) + at.c, at.have, f);
@@ -246,8 +246,8 @@ __global__ __launch_bounds__(GN_T) void gn_grad_sums_kernel(Rows<const T> dy, Ro
                 if (r + j * at.step >= s1) break;
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    const float xh = (act_f<PRE>((float)u[j][v]) - mean[v]) * rstd[v];
-                    const float dz = (float)d[j][v] * act_grad_f<POST>(fmaf(xh, ga[v], be[v]));
+                    const float xh = (act_f<PRE, fine<T>()>((float)u[j][v]) - mean[v]) * rstd[v];
+                    const float dz = (float)d[j][v] * act_grad_f<POST, fine<T>()>(fmaf(xh, ga[v], be[v]));
                     a1[v] += dz;
                     a2[v] = fmaf(dz, xh, a2[v]);
                 }
@@ -353,9 +353,9 @@ __global__ __launch_bounds__(GN_T) void gn_dx_kernel(Rows<const T> dy, Rows<cons
             float f[V];
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const float xv = (float)u[j][v], xh = (act_f<PRE>(xv) - mean[v]) * rstd[v];
-                const float dz = (float)d[j][v] * act_grad_f<POST>(fmaf(xh, ga[v], be[v]));
-                f[v] = rstd[v] * (fmaf(dz, ga[v], -c1[v]) - xh * c2[v]) * act_grad_f<PRE>(xv);
+                const float xv = (float)u[j][v], xh = (act_f<PRE, fine<T>()>(xv) - mean[v]) * rstd[v];
+                const float dz = (float)d[j][v] * act_grad_f<POST, fine<T>()>(fmaf(xh, ga[v], be[v]));
+                f[v] = rstd[v] * (fmaf(dz, ga[v], -c1[v]) - xh * c2[v]) * act_grad_f<PRE, fine<T>()>(xv);
                 if (s >= n) f[v] = 0.f;
             }
             gn_store<V>(dx.at(at.b, s) + at.c, at.have, f);
@@ -374,8 +374,8 @@ static inline GnPlan gn_plan(int B, int S, int C, int G, int bytes) {
     pl.width = pl.lanes * V;
     pl.slices = (vecs + pl.lanes - 1) / pl.lanes;
     pl.local = std::min(G, (pl.width + pl.D - 2) / pl.D + 1);
-    // 4 workgroups a CU, each with 16 frames a thread at least
-    const int least = 16 * GN_T / pl.lanes;
+    // 8 workgroups a CU, each with 4 frames a thread at least
+    const int least = 4 * GN_T / pl.lanes;
     const long want = std::max(1l, 2048 / ((long)B * pl.slices));
     pl.rows = (int)std::min<long>(std::max<long>(least, (S + want - 1) / want), GN_ROWS * GN_T / pl.lanes);
     pl.chunks = (S + pl.rows - 1) / pl.rows;

@@ -6,6 +6,8 @@
 // over the registers gives every h_t.  x and gate are read once and h is written once.  The gradient is the same recurrence
 // from the last frame back, E_t = a_t (dh_t + E_{t+1}); the h_{t-1} that dgate needs are scanned again within 32 frames from
 // a state that the forward pass saved, which costs 1/32 of a row per frame instead of reading h, and keeps them in 32 bits.
+// 1 - a comes from e^-gate, and h from a h + (1 - a) x: the shorter x + a (h - x) rounds at the size of x, which a gate near 1
+// lets through to a state that is far smaller.
 // t counts frames in walking order; frame s is t, or S - 1 - t in reverse.  Frames past an utterance's end count as a = 1, B = 0.
 #pragma once
 #include <algorithm>
@@ -14,22 +16,30 @@
 namespace msf2 {
 
 constexpr int REC_SAVE = MSF2_RECURRENCE_SAVE;
-constexpr int REC_LC = 16;                   // lanes side by side over channels; the four rows of lanes of a wave follow in time
-constexpr int REC_LT = 64 / REC_LC;
-constexpr int REC_WIDE = 8;                  // waves of a workgroup, where a sequence is longer than one wave's frames
+constexpr int REC_WIDE = 8;                  // waves of a workgroup, where a sequence is longer than the short form's frames
 
 // How the work is dealt out: `slices` of channels by `pieces` of `piece` frames by utterances.
 struct RecPlan {
-    int slices, pieces, waves;
-    long piece;
+    int lanes, slices, pieces, waves, piece;
+    bool near;                               // a tile's rows span less than 2^32 bytes in every operand
+};
+
+// The lanes of a workgroup: LC side by side over V channels each, the LT = 64 / LC groups of a wave one after the other in time,
+// R frames a thread, W waves.
+template <class T_, int V_, int LC_, int R_, int W_> struct RecShape {
+    typedef T_ T;
+    typedef typename VecOf<T_, V_>::type vec;
+    static constexpr int V = V_, LC = LC_, LT = 64 / LC_, R = R_, W = W_;
+    static constexpr int WAVE = LT * R, TILE = WAVE * W;       // frames of a wave, of a workgroup
+    static_assert(LC == 16 || LC == 32 || LC == 64, "the scans are over rows of 16 lanes or halves of a wave");
 };
 
 // What a workgroup works on, and a thread's place in it.  The lane of the last channels is moved left to end with the
 // row, so that every load is a whole vector; what it shares with its neighbour is computed twice and written once (`own` on).
 // Slices of the same frames share lines where rows are not aligned to them, and go to the same XCD one after the other: blocks are dealt
 // to the 8 XCDs in turn, so block i of XCD k takes the i-th of the k-th eighth of the work.
-template <int V> struct RecPlace {
-    int b, p, n, tl, wave, c, own;
+template <class Q> struct RecPlace {
+    int b, p, n, tl, cl, wave, c, own;
     bool whole;                              // no lane of the workgroup is past the row's end
     __device__ RecPlace(const RecPlan& pl, const int* lengths, int S, int C) {
         const unsigned each = gridDim.x / 8, more = gridDim.x % 8, xcd = blockIdx.x % 8;
@@ -41,12 +51,14 @@ template <int V> struct RecPlace {
         n = frames_of(lengths, b, S);
         const int lane = threadIdx.x & 63;
         wave = threadIdx.x >> 6;
-        tl = lane / REC_LC;
-        const int c0 = (slice * REC_LC + lane % REC_LC) * V;
-        c = min(c0, C - V);
+        tl = lane / Q::LC;
+        cl = lane % Q::LC;
+        const int c0 = (slice * Q::LC + cl) * Q::V;
+        c = min(c0, C - Q::V);
         own = c0 - c;                        // V and more: nothing is this lane's own
-        whole = (slice + 1) * REC_LC * V <= C;
+        whole = (slice + 1) * Q::LC * Q::V <= C;
     }
+    __device__ __forceinline__ bool first() const { return wave == 0 && tl == 0; }
 };
 
 // Runs of V neighbouring channels.
@@ -70,9 +82,10 @@ template <int V> struct Run {
     }
 };
 
-// One level of a scan over the rows of 16 lanes: every lane gets the run of the earlier (lo) and of the later (hi) half of its
-// pair, rows 2k and 2k + 1 with D = 16, the two halves of the wave with D = 32.  v_permlane*_swap exchanges the odd half of its
-// first register with the even half of its second, so with the same value in both it leaves lo in the first, hi in the second.
+// One level of a scan over the lanes of a wave: every lane gets the run of the earlier (lo) and of the later (hi) half of its
+// pair, rows of 16 lanes 2k and 2k + 1 with D = 16, the two halves of the wave with D = 32.  v_permlane*_swap exchanges the odd half
+// of its first register with the even half of its second, so with the same value in both it leaves lo in the first, hi in the
+// second.
 template <int D, int V> __device__ __forceinline__ void halves(const Run<V>& r, Run<V>& lo, Run<V>& hi) {
     auto swap = [](float f, float& l, float& h) {
         const unsigned u = __builtin_bit_cast(unsigned, f);
@@ -88,75 +101,51 @@ template <int D, int V> __device__ __forceinline__ void halves(const Run<V>& r, 
 }
 // From each time lane's run: `before`, the run of all earlier lanes of the wave, and `all`, the run of the whole wave, in
 // every lane.  BACK: later lanes come first.
-template <bool BACK, int V> __device__ __forceinline__ void wave_scan(const Run<V>& r, int tl, Run<V>& before, Run<V>& all) {
-    Run<V> lo, hi, pair;
-    halves<16, V>(r, lo, hi);
-    const bool second = BACK ? !(tl & 1) : tl & 1, late = BACK ? tl < 2 : tl >= 2;
-    const Run<V>&first = BACK ? hi : lo, &then = BACK ? lo : hi;
+template <bool BACK, int LC, int V> __device__ __forceinline__ void wave_scan(const Run<V>& r, int tl, Run<V>& before, Run<V>& all) {
+    Run<V> lo, hi, part;
+    auto pick = [&](bool on) {               // the run of the half that comes first, for the lanes of the other
+        Run<V> o;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        before.a[v] = second ? first.a[v] : 1.f;
-        before.b[v] = second ? first.b[v] : 0.f;
+        for (int v = 0; v < V; ++v) {
+            o.a[v] = on ? (BACK ? hi : lo).a[v] : 1.f;
+            o.b[v] = on ? (BACK ? hi : lo).b[v] : 0.f;
+        }
+        return o;
+    };
+    part = r;
+    before.clear();
+    if constexpr (LC == 64) {                // a wave is one frame wide
+        all = r;
+        return;
     }
-    pair = then;
-    pair.after(first);
-    halves<32, V>(pair, lo, hi);
-    Run<V> skip;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        skip.a[v] = late ? first.a[v] : 1.f;
-        skip.b[v] = late ? first.b[v] : 0.f;
+    if constexpr (LC == 16) {
+        halves<16, V>(part, lo, hi);
+        before = pick(BACK ? !(tl & 1) : tl & 1);
+        part = BACK ? lo : hi;
+        part.after(BACK ? hi : lo);
     }
-    before.after(skip);
-    all = then;
-    all.after(first);
+    halves<32, V>(part, lo, hi);
+    const Run<V> skip = pick(BACK ? tl < 32 / LC : tl >= 32 / LC);
+    if constexpr (LC == 16) before.after(skip);
+    else before = skip;
+    all = BACK ? lo : hi;
+    all.after(BACK ? hi : lo);
 }
 
 // The waves of a workgroup in turn: h, the state before the tile, becomes the state after it, and `mine` the one before this
-// wave's frames.  `runs` is one of two buffers that tiles take in turn, so one barrier a tile is enough: who fills a buffer
-// again has passed the barrier of the tile between, which nobody passes before having read it.
-template <bool BACK, int V, int W>
-__device__ __forceinline__ void join_waves(const Run<V>& all, int wave, int tl, Run<V> (*runs)[REC_LC], float (&h)[V], float (&mine)[V]) {
-    const int cl = threadIdx.x & (REC_LC - 1);
-    if constexpr (W == 1) {
+// wave's frames.  The runs lie in one of two buffers that tiles take in turn, so one barrier a tile is enough: who fills a
+// buffer again has passed the barrier of the tile between, which nobody passes before having read it.
+template <bool BACK, class Q>
+__device__ __forceinline__ void join_waves(const Run<Q::V> (*runs)[Q::LC], int wave, int cl, float (&h)[Q::V], float (&mine)[Q::V]) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) mine[v] = h[v];
-        all.apply(h);
-        return;
-    }
-    if (tl == 0) runs[wave][cl] = all;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < W; ++k) {
-        const int w = BACK ? W - 1 - k : k;
+    for (int k = 0; k < Q::W; ++k) {
+        const int w = BACK ? Q::W - 1 - k : k;
         if (w == wave) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) mine[v] = h[v];
+            for (int v = 0; v < Q::V; ++v) mine[v] = h[v];
         }
         runs[w][cl].apply(h);
     }
-}
-
-// The gate: a = 1 / (1 + t) and na = 1 - a = t a, t = e^-g.  1 - a has to come from t, and h from a h + (1 - a) x: the shorter
-// x + a (h - x) rounds at the size of x, which a gate near 1 lets through to a state that is far smaller.  A rounding d of g log2 e is a
-// relative error d ln 2 of t, all of which 1 - a takes: FINE (fp32) adds the part that the product's rounding left out.  Gates beyond 87
-// are held there (e^87 and its inverse are normal numbers; max and min keep NaN).
-template <bool FINE> __device__ __forceinline__ void rec_gate(float g, float& a, float& na) {
-    constexpr float LOG2E = 1.44269504088896f, LN2 = 0.693147180559945f;
-    g = __builtin_elementwise_maximum(g, -87.f);
-    if constexpr (FINE) g = __builtin_elementwise_minimum(g, 87.f);
-    const float u = -g * LOG2E;
-    float t = __builtin_amdgcn_exp2f(u);
-    if constexpr (FINE) t = fmaf(t * LN2, fmaf(-g, LOG2E, -u), t);
-    a = __builtin_amdgcn_rcpf(1.f + t);
-    na = t * a;
-}
-template <class T> constexpr bool rec_fine() { return sizeof(T) == 4; }
-
-// Frames outside the utterance: a gate of 87 is a = 1 exactly, and nothing is added.
-template <int V, class T> __device__ __forceinline__ void rec_shut(typename VecOf<T, V>::type& g) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) g[v] = (T)87.f;
 }
 
 template <int V, class T> __device__ __forceinline__ void rec_store(T* row, int own, const float (&f)[V]) {
@@ -174,49 +163,105 @@ template <int V> __device__ __forceinline__ void rec_read(const float* p, float 
     for (int v = 0; v < V; ++v) f[v] = u[v];
 }
 
-// The state before piece p: `start` and the runs of the pieces before it (BACK: behind it), agg [b][pieces][2][C].
-template <bool BACK, int V>
-__device__ __forceinline__ void rec_carry(const RecPlan& pl, const float* agg, const float* start, int b, int p, int c, int C, float (&h)[V]) {
+// The state before piece p in every lane: `start` and the runs of the pieces before it (BACK: behind it), agg
+// [b][pieces][2][C].  The time lanes and waves take a share of the pieces each, joined like the frames of a tile.
+template <bool BACK, class Q>
+__device__ __forceinline__ void rec_carry(const RecPlan& pl, const float* agg, const float* start, const RecPlace<Q>& at, int C,
+                                          Run<Q::V> (*runs)[Q::LC], float (&h)[Q::V]) {
+    constexpr int V = Q::V, SHARES = Q::W * Q::LT;
 #pragma unroll
     for (int v = 0; v < V; ++v) h[v] = 0.f;
-    if (start) rec_read<V>(start + (long)b * C + c, h);
-    const int k0 = BACK ? pl.pieces - 1 : 0, n = BACK ? pl.pieces - 1 - p : p;
-    for (int k = 0; k < n; ++k) {
-        const float* q = agg + ((long)b * pl.pieces + (BACK ? k0 - k : k)) * 2 * C + c;
-        Run<V> r;
-        rec_read<V>(q, r.a);
-        rec_read<V>(q + C, r.b);
-        r.apply(h);
+    if (start) rec_read<V>(start + (long)at.b * C + at.c, h);
+    const int count = BACK ? pl.pieces - 1 - at.p : at.p;
+    if (pl.pieces == 1 || count == 0) return;        // the same for the whole workgroup
+    const int share = (count + SHARES - 1) / SHARES, place = at.wave * Q::LT + at.tl;
+    const int from = BACK ? at.p + 1 : 0;            // BACK: the last piece comes first, and so does the last lane
+    const int k0 = min(place * share, count), k1 = min(k0 + share, count);
+    Run<V> r, before, all;
+    r.clear();
+#pragma unroll 4
+    for (int i = 0; i < k1 - k0; ++i) {
+        const float* q = agg + ((long)at.b * pl.pieces + from + (BACK ? k1 - 1 - i : k0 + i)) * 2 * C + at.c;
+        Run<V> next;
+        rec_read<V>(q, next.a);
+        rec_read<V>(q + C, next.b);
+        next.after(r);
+        r = next;
     }
+    wave_scan<BACK, Q::LC, V>(r, at.tl, before, all);
+    if (at.tl == 0) runs[at.wave][at.cl] = all;
+    __syncthreads();
+    float mine[V];
+    join_waves<BACK, Q>(runs, at.wave, at.cl, h, mine);
 }
 
-// A thread's R frames of a tile; which of them are in the utterance, and whether all of the tile's are.
-template <int R> struct RecFrames {
-    long t, s0;
-    int n, step;
-    bool all;
-    // first: this thread's first frame walked; tile, rows: the workgroup's
-    __device__ __forceinline__ RecFrames(long first, long tile, int rows, long end, int n_, int S, int reverse) : t(first), n(n_) {
-        s0 = reverse ? S - 1 - t : t;
-        step = reverse ? -1 : 1;
-        all = tile + rows <= end && (reverse ? tile >= S - n : tile + rows <= n);
+// Where a tile's frames lie.  `all`: every one of them is in the utterance, and then a thread's row j is at an address that is the same for
+// the workgroup up to a 32-bit offset of the thread's own: the compiler keeps the one in scalar registers, and a load costs no vector
+// arithmetic.  At the ends each row has its own address, held to the utterance (to memory, at least), and frames outside it are
+// a = 1 and add nothing, whatever memory holds there.
+template <class Q> struct RecFrames {
+    int t, first, n, S, end;                 // the tile's and this thread's first frame walked; no frame from `end` on
+    bool reverse, all;
+    __device__ __forceinline__ RecFrames(int tile, int mine, int end_, int n_, int S_, bool reverse_, bool near)
+        : t(tile), first(tile + mine), n(n_), S(S_), end(end_), reverse(reverse_) {
+        all = near && tile + Q::TILE <= end && (reverse ? tile >= S - n : tile + Q::TILE <= n);
     }
-    __device__ __forceinline__ long s(int j) const { return s0 + step * j; }
-    __device__ __forceinline__ bool live(int j) const { return s(j) >= 0 && s(j) < n; }
-    __device__ __forceinline__ long held(int j) const { return min(max(s(j), 0l), (long)max(n - 1, 0)); }   // in memory at least
+    __device__ __forceinline__ int s(int j) const { return reverse ? S - 1 - first - j : first + j; }
+    __device__ __forceinline__ bool live(int j) const { return first + j < end && s(j) < n; }
+    __device__ __forceinline__ int held(int j) const { return min(max(s(j), 0), max(n - 1, 0)); }
+};
+// One operand's rows: utterance b, and this thread's offset in bytes within a tile.
+template <class Q, class U> struct RecRows {
+    U* p;
+    long row;
+    unsigned mine;
+    int c;
+    __device__ __forceinline__ RecRows(const Rows<U>& r, int b, int mine_, int c_, bool reverse) : p(r.p + b * r.batch), row(r.row), c(c_) {
+        mine = (unsigned)(((long)(reverse ? Q::TILE - Q::R - mine_ : mine_) * r.row + c_) * (long)sizeof(U));
+    }
+    // the address of row j without this thread's offset, for a whole tile
+    __device__ __forceinline__ U* base(const RecFrames<Q>& fr, int j) const {
+        return p + (long)(fr.reverse ? fr.S - fr.t - Q::TILE + Q::R - 1 - j : fr.t + j) * row;
+    }
+    template <class B> static __device__ __forceinline__ B* off(B* q, unsigned bytes) {
+        return reinterpret_cast<B*>(reinterpret_cast<std::conditional_t<std::is_const<B>::value, const char, char>*>(q) + bytes);
+    }
+    __device__ __forceinline__ void load(const RecFrames<Q>& fr, typename Q::vec (&v)[Q::R]) const {
+        if (fr.all) {
+#pragma unroll
+            for (int j = 0; j < Q::R; ++j) v[j] = load_vec<Q::V>(off(base(fr, j), mine));
+        } else {
+#pragma unroll
+            for (int j = 0; j < Q::R; ++j) v[j] = load_vec<Q::V>(p + (long)fr.held(j) * row + c);
+        }
+    }
+    __device__ __forceinline__ void store(const RecFrames<Q>& fr, bool whole, int own, float (&f)[Q::R][Q::V]) const {
+        if (fr.all && whole) {
+#pragma unroll
+            for (int j = 0; j < Q::R; ++j) store_vec<Q::V, true>(off(base(fr, j), mine), f[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < Q::R; ++j)
+                if (fr.first + j < fr.end) {
+#pragma unroll
+                    for (int v = 0; v < Q::V; ++v) f[j][v] = fr.live(j) ? f[j][v] : 0.f;
+                    rec_store<Q::V>(p + (long)fr.s(j) * row + c, own, f[j]);
+                }
+        }
+    }
 };
 
 // The run of one piece, for sequences too few to fill the chip: agg, and `start` copied to `kept`, because the pieces of the
 // next launch read it while one of them may write the last state into the same memory.  u is x, or dh with BACK; a thread
-// walks piece / (W REC_LT) frames on end.
-template <bool BACK, class T, int V, int W>
-__global__ __launch_bounds__(64 * W) void rec_piece_kernel(Rows<const T> u, Rows<const T> gate, const float* start, const int* lengths,
-                                                           float* agg, float* kept, RecPlan pl, int S, int C, int reverse) {
-    constexpr int R = 8;
-    __shared__ Run<V> runs[W][REC_LC];
-    const RecPlace<V> at(pl, lengths, S, C);
-    const bool writes = at.wave == 0 && at.tl == 0;
-    if (at.p == (BACK ? pl.pieces - 1 : 0) && writes) {
+// walks piece / (W LT) frames on end.
+template <bool BACK, class Q>
+__global__ __launch_bounds__(64 * Q::W) void rec_piece_kernel(Rows<const typename Q::T> u, Rows<const typename Q::T> gate, const float* start,
+                                                              const int* lengths, float* agg, float* kept, RecPlan pl, int S, int C, bool reverse) {
+    typedef typename Q::T T;
+    constexpr int V = Q::V, R = 8;
+    __shared__ Run<V> runs[Q::W][Q::LC];
+    const RecPlace<Q> at(pl, lengths, S, C);
+    if (at.p == (BACK ? pl.pieces - 1 : 0) && at.first()) {
         float h[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) h[v] = 0.f;
@@ -224,40 +269,40 @@ __global__ __launch_bounds__(64 * W) void rec_piece_kernel(Rows<const T> u, Rows
         rec_store<V>(kept + (long)at.b * C + at.c, at.own, h);
     }
     if (at.p == (BACK ? 0 : pl.pieces - 1)) return;         // nothing follows it
-    const int steps = (int)(pl.piece / (W * REC_LT));       // a multiple of R
-    const long t0 = at.p * pl.piece + (long)(at.wave * REC_LT + at.tl) * steps;
+    const int steps = pl.piece / (Q::W * Q::LT);            // a multiple of R
+    const int t0 = at.p * pl.piece + (at.wave * Q::LT + at.tl) * steps, cap = max(at.n - 1, 0);
+    const T *up = u.at(at.b, 0) + at.c, *gp = gate.at(at.b, 0) + at.c;
     Run<V> r;
     r.clear();
     for (int k = 0; k < steps; k += R) {
-        const RecFrames<R> fr(BACK ? t0 + steps - R - k : t0 + k, 0, 0, 0, at.n, S, reverse);
-        typename VecOf<T, V>::type uv[R], gv[R];
+        typename Q::vec uv[R], gv[R];
+        bool live[R];
 #pragma unroll
         for (int j = 0; j < R; ++j) {
-            uv[j] = load_vec<V>(u.at(at.b, fr.held(j)) + at.c);
-            gv[j] = load_vec<V>(gate.at(at.b, fr.held(j)) + at.c);
+            const int t = t0 + (BACK ? steps - 1 - k - j : k + j), s = reverse ? S - 1 - t : t, h = min(max(s, 0), cap);
+            live[j] = t < S && s < at.n;
+            uv[j] = load_vec<V>(up + (long)h * u.row);
+            gv[j] = load_vec<V>(gp + (long)h * gate.row);
         }
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const int j = BACK ? R - 1 - i : i;
-            if (!fr.live(j) || fr.t + j >= S) rec_shut<V, T>(gv[j]), uv[j] = 0;
+        for (int j = 0; j < R; ++j)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 float a, na;
-                rec_gate<rec_fine<T>()>((float)gv[j][v], a, na);
-                const float f = (float)uv[j][v];
+                sigmoid_pair<fine<T>()>(live[j] ? (float)gv[j][v] : 87.f, a, na);       // 87: a is 1
+                const float f = live[j] ? (float)uv[j][v] : 0.f;
                 r.b[v] = BACK ? a * (r.b[v] + f) : fmaf(a, r.b[v], na * f);
                 r.a[v] *= a;
             }
-        }
     }
     Run<V> before, all;
-    wave_scan<BACK, V>(r, at.tl, before, all);
-    if (at.tl == 0) runs[at.wave][threadIdx.x & (REC_LC - 1)] = all;
+    wave_scan<BACK, Q::LC, V>(r, at.tl, before, all);
+    if (at.tl == 0) runs[at.wave][at.cl] = all;
     __syncthreads();
-    if (writes) {
+    if (at.first()) {
         r.clear();
-        for (int k = 0; k < W; ++k) {
-            Run<V> next = runs[BACK ? W - 1 - k : k][threadIdx.x];
+        for (int k = 0; k < Q::W; ++k) {
+            Run<V> next = runs[BACK ? Q::W - 1 - k : k][at.cl];
             next.after(r);
             r = next;
         }
@@ -267,122 +312,112 @@ __global__ __launch_bounds__(64 * W) void rec_piece_kernel(Rows<const T> u, Rows
     }
 }
 
-template <class T, int V, int R, int W>
-__global__ __launch_bounds__(64 * W) void rec_forward_kernel(Rows<const T> x, Rows<const T> gate, const float* start, const int* lengths,
-                                                             Rows<T> h, float* last, float* saved, const float* agg, RecPlan pl,
-                                                             int S, int C, int reverse) {
-    constexpr int TILE = W * REC_LT * R;
-    __shared__ Run<V> runs[2][W][REC_LC];
-    const RecPlace<V> at(pl, lengths, S, C);
-    const long t0 = at.p * pl.piece, t1 = min(t0 + pl.piece, (long)S);
-    const int blocks = (S + REC_SAVE - 1) / REC_SAVE;
-    const int mine = (at.wave * REC_LT + at.tl) * R;           // this thread's first frame in a tile
-    typedef typename VecOf<T, V>::type vec;
-    vec nx[R], ng[R];
-    auto fetch = [&](long t) {
-        const RecFrames<R> fr(t + mine, t, TILE, t1, at.n, S, reverse);
+// Frames outside the utterance: a gate of 87 is a = 1 exactly, and nothing is added.
+template <class Q> __device__ __forceinline__ void rec_mask(const RecFrames<Q>& fr, typename Q::vec (&v)[Q::R], float with) {
 #pragma unroll
-        for (int j = 0; j < R; ++j) {
-            nx[j] = load_vec<V>(x.at(at.b, fr.held(j)) + at.c);
-            ng[j] = load_vec<V>(gate.at(at.b, fr.held(j)) + at.c);
-        }
+    for (int j = 0; j < Q::R; ++j)
+        if (!fr.live(j))
+#pragma unroll
+            for (int i = 0; i < Q::V; ++i) v[j][i] = (typename Q::T)with;
+}
+
+template <class Q>
+__global__ __launch_bounds__(64 * Q::W) void rec_forward_kernel(Rows<const typename Q::T> x_, Rows<const typename Q::T> gate_, const float* start,
+                                                                const int* lengths, Rows<typename Q::T> h_, float* last, float* saved,
+                                                                const float* agg, RecPlan pl, int S, int C, bool reverse) {
+    typedef typename Q::T T;
+    constexpr int V = Q::V, R = Q::R;
+    __shared__ Run<V> runs[2][Q::W][Q::LC];
+    const RecPlace<Q> at(pl, lengths, S, C);
+    const int t0 = at.p * pl.piece, t1 = min(t0 + pl.piece, S), blocks = (S + REC_SAVE - 1) / REC_SAVE;
+    const int mine = at.wave * Q::WAVE + at.tl * R;            // this thread's first frame in a tile
+    const RecRows<Q, const T> x(x_, at.b, mine, at.c, reverse), gate(gate_, at.b, mine, at.c, reverse);
+    const RecRows<Q, T> h(h_, at.b, mine, at.c, reverse);
+    typename Q::vec nx[R], ng[R];
+    auto fetch = [&](int t) {
+        const RecFrames<Q> fr(t, mine, t1, at.n, S, reverse, pl.near);
+        x.load(fr, nx);
+        gate.load(fr, ng);
     };
     fetch(t0);
     float carry[V];
-    rec_carry<false, V>(pl, agg, start, at.b, at.p, at.c, C, carry);
-    int turn = 0;
-    for (long t = t0; t < t1; t += TILE, turn ^= 1) {
-        const RecFrames<R> fr(t + mine, t, TILE, t1, at.n, S, reverse);
+    rec_carry<false, Q>(pl, agg, start, at, C, runs[0], carry);
+    int turn = 1;
+    for (int t = t0; t < t1; t += Q::TILE, turn ^= 1) {
+        const RecFrames<Q> fr(t, mine, t1, at.n, S, reverse, pl.near);
         float a[R][V], f[R][V];
         Run<V> r, before, all;
         r.clear();
-        if (!fr.all) {
-#pragma unroll
-            for (int j = 0; j < R; ++j)
-                if (!fr.live(j) || fr.t + j >= t1) rec_shut<V, T>(ng[j]), nx[j] = 0;
-        }
+        if (!fr.all) rec_mask<Q>(fr, nx, 0.f), rec_mask<Q>(fr, ng, 87.f);
 #pragma unroll
         for (int j = 0; j < R; ++j)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 float na;
-                rec_gate<rec_fine<T>()>((float)ng[j][v], a[j][v], na);
+                sigmoid_pair<fine<T>()>((float)ng[j][v], a[j][v], na);
                 f[j][v] = na * (float)nx[j][v];
                 r.b[v] = fmaf(a[j][v], r.b[v], f[j][v]);
                 r.a[v] *= a[j][v];
             }
-        if (t + TILE < t1) fetch(t + TILE);
-        wave_scan<false, V>(r, at.tl, before, all);
+        if (t + Q::TILE < t1) fetch(t + Q::TILE);
+        wave_scan<false, Q::LC, V>(r, at.tl, before, all);
+        if (at.tl == 0) runs[turn][at.wave][at.cl] = all;
+        __syncthreads();
         float hv[V];
-        join_waves<false, V, W>(all, at.wave, at.tl, runs[turn], carry, hv);
+        join_waves<false, Q>(runs[turn], at.wave, at.cl, carry, hv);
         before.apply(hv);
-        if (saved && fr.t % REC_SAVE == 0 && fr.t < t1)
-            rec_store<V>(saved + ((long)at.b * blocks + fr.t / REC_SAVE) * C + at.c, at.own, hv);
+        if (saved && fr.first % REC_SAVE == 0 && fr.first < t1)
+            rec_store<V>(saved + ((long)at.b * blocks + fr.first / REC_SAVE) * C + at.c, at.own, hv);
 #pragma unroll
         for (int j = 0; j < R; ++j)
 #pragma unroll
             for (int v = 0; v < V; ++v) f[j][v] = hv[v] = fmaf(a[j][v], hv[v], f[j][v]);
-        if (fr.all && at.whole) {
-#pragma unroll
-            for (int j = 0; j < R; ++j) store_vec<V>(h.at(at.b, fr.s(j)) + at.c, f[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < R; ++j)
-                if (fr.t + j < t1) {
-#pragma unroll
-                    for (int v = 0; v < V; ++v) f[j][v] = fr.live(j) ? f[j][v] : 0.f;
-                    rec_store<V>(h.at(at.b, fr.s(j)) + at.c, at.own, f[j]);
-                }
-        }
+        h.store(fr, at.whole, at.own, f);
     }
-    if (last && t1 == S && at.wave == 0 && at.tl == 0) rec_store<V>(last + (long)at.b * C + at.c, at.own, carry);
+    if (last && t1 == S && at.first()) rec_store<V>(last + (long)at.b * C + at.c, at.own, carry);
 }
 
-template <class T, int V, int R, int W>
-__global__ __launch_bounds__(64 * W) void rec_backward_kernel(Rows<const T> dh, Rows<const T> x, Rows<const T> gate, const float* saved,
-                                                              const float* start, const int* lengths, Rows<T> dx, Rows<T> dgate,
-                                                              float* dh0, const float* agg, RecPlan pl, int S, int C, int reverse) {
-    constexpr int TILE = W * REC_LT * R;
-    static_assert(REC_LT * R % REC_SAVE == 0, "a wave's frames begin at a saved state");
-    __shared__ Run<V> runs[2][W][REC_LC];
-    const RecPlace<V> at(pl, lengths, S, C);
-    const long t0 = at.p * pl.piece, t1 = min(t0 + pl.piece, (long)S);
-    const int blocks = (S + REC_SAVE - 1) / REC_SAVE;
-    const int mine = (at.wave * REC_LT + at.tl) * R;
-    typedef typename VecOf<T, V>::type vec;
-    vec nd[R], nx[R], ng[R];
+template <class Q>
+__global__ __launch_bounds__(64 * Q::W) void rec_backward_kernel(Rows<const typename Q::T> dh_, Rows<const typename Q::T> x_,
+                                                                 Rows<const typename Q::T> gate_, const float* saved, const float* start,
+                                                                 const int* lengths, Rows<typename Q::T> dx_, Rows<typename Q::T> dgate_, float* dh0,
+                                                                 const float* agg, RecPlan pl, int S, int C, bool reverse) {
+    typedef typename Q::T T;
+    constexpr int V = Q::V, R = Q::R;
+    constexpr int SHARE = Q::WAVE < REC_SAVE ? REC_SAVE / Q::WAVE : 1;       // waves that start from the same saved state
+    static_assert(Q::TILE % REC_SAVE == 0 && (SHARE > 1 || Q::WAVE % REC_SAVE == 0), "a tile begins at a saved state");
+    __shared__ Run<V> runs[2][Q::W][Q::LC], ahead[2][SHARE > 1 ? Q::W : 1][Q::LC];
+    const RecPlace<Q> at(pl, lengths, S, C);
+    const int t0 = at.p * pl.piece, t1 = min(t0 + pl.piece, S), blocks = (S + REC_SAVE - 1) / REC_SAVE;
+    const int mine = at.wave * Q::WAVE + at.tl * R;
+    const RecRows<Q, const T> dh(dh_, at.b, mine, at.c, reverse), x(x_, at.b, mine, at.c, reverse), gate(gate_, at.b, mine, at.c, reverse);
+    const RecRows<Q, T> dx(dx_, at.b, mine, at.c, reverse), dgate(dgate_, at.b, mine, at.c, reverse);
+    typename Q::vec nd[R], nx[R], ng[R];
     float nh[V];
-    auto fetch = [&](long t) {
-        const RecFrames<R> fr(t + mine, t, TILE, t1, at.n, S, reverse);
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-            nd[j] = load_vec<V>(dh.at(at.b, fr.held(j)) + at.c);
-            nx[j] = load_vec<V>(x.at(at.b, fr.held(j)) + at.c);
-            ng[j] = load_vec<V>(gate.at(at.b, fr.held(j)) + at.c);
-        }
-        const long block = min((t + at.wave * (REC_LT * R)) / REC_SAVE, (long)blocks - 1);      // the wave's first frame
+    auto fetch = [&](int t) {
+        const RecFrames<Q> fr(t, mine, t1, at.n, S, reverse, pl.near);
+        dh.load(fr, nd);
+        x.load(fr, nx);
+        gate.load(fr, ng);
+        const int block = min((t + at.wave * Q::WAVE) / REC_SAVE, blocks - 1);
         rec_read<V>(saved + ((long)at.b * blocks + block) * C + at.c, nh);
     };
-    const long tiles = (t1 - t0 + TILE - 1) / TILE;
-    fetch(t0 + (tiles - 1) * TILE);
+    const int tiles = (t1 - t0 + Q::TILE - 1) / Q::TILE;
+    fetch(t0 + (tiles - 1) * Q::TILE);
     float carry[V];
-    rec_carry<true, V>(pl, agg, start, at.b, at.p, at.c, C, carry);
-    int turn = 0;
-    for (long t = t0 + (tiles - 1) * TILE; t >= t0; t -= TILE, turn ^= 1) {
-        const RecFrames<R> fr(t + mine, t, TILE, t1, at.n, S, reverse);
-        float a[R][V], na[R][V], f[R][V], d[R][V], hv[V];
-        Run<V> r, q, before, all;
+    rec_carry<true, Q>(pl, agg, start, at, C, runs[0], carry);
+    int turn = 1;
+    for (int t = t0 + (tiles - 1) * Q::TILE; t >= t0; t -= Q::TILE, turn ^= 1) {
+        const RecFrames<Q> fr(t, mine, t1, at.n, S, reverse, pl.near);
+        float a[R][V], na[R][V], f[R][V], d[R][V], hv[V], e[V];
+        Run<V> r, q, before, behind, all;
         r.clear();
-        if (!fr.all) {
-#pragma unroll
-            for (int j = 0; j < R; ++j)
-                if (!fr.live(j) || fr.t + j >= t1) rec_shut<V, T>(ng[j]), nx[j] = 0, nd[j] = 0;
-        }
+        if (!fr.all) rec_mask<Q>(fr, nd, 0.f), rec_mask<Q>(fr, nx, 0.f), rec_mask<Q>(fr, ng, 87.f);
 #pragma unroll
         for (int j = 0; j < R; ++j)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                rec_gate<rec_fine<T>()>((float)ng[j][v], a[j][v], na[j][v]);
+                sigmoid_pair<fine<T>()>((float)ng[j][v], a[j][v], na[j][v]);
                 f[j][v] = (float)nx[j][v];
                 d[j][v] = (float)nd[j][v];
                 r.b[v] = fmaf(a[j][v], r.b[v], na[j][v] * f[j][v]);
@@ -396,9 +431,20 @@ __global__ __launch_bounds__(64 * W) void rec_backward_kernel(Rows<const T> dh, 
 #pragma unroll
             for (int j = R - 1; j >= 0; --j) q.b[v] = a[j][v] * (d[j][v] + q.b[v]);
         }
-        if (t > t0) fetch(t - TILE);
-        wave_scan<false, V>(r, at.tl, before, all);
+        if (t > t0) fetch(t - Q::TILE);
+        wave_scan<false, Q::LC, V>(r, at.tl, before, all);
+        if (SHARE > 1 && at.tl == 0) ahead[turn][at.wave][at.cl] = all;
+        wave_scan<true, Q::LC, V>(q, at.tl, behind, all);
+        if (at.tl == 0) runs[turn][at.wave][at.cl] = all;
+        __syncthreads();
+        join_waves<true, Q>(runs[turn], at.wave, at.cl, carry, e);
+        if constexpr (SHARE > 1) {
+#pragma unroll
+            for (int k = 1; k < SHARE; ++k)
+                if (at.wave % SHARE >= k) ahead[turn][at.wave / SHARE * SHARE + k - 1][at.cl].apply(hv);
+        }
         before.apply(hv);
+        behind.apply(e);
         // f becomes (1 - a_t) (h_{t-1} - x_t)
 #pragma unroll
         for (int j = 0; j < R; ++j)
@@ -408,10 +454,6 @@ __global__ __launch_bounds__(64 * W) void rec_backward_kernel(Rows<const T> dh, 
                 f[j][v] = na[j][v] * (hv[v] - xv);
                 hv[v] = fmaf(a[j][v], hv[v], na[j][v] * xv);
             }
-        wave_scan<true, V>(q, at.tl, before, all);
-        float e[V];
-        join_waves<true, V, W>(all, at.wave, at.tl, runs[turn], carry, e);
-        before.apply(e);
         // d becomes dx, f becomes dgate
 #pragma unroll
         for (int j = R - 1; j >= 0; --j)
@@ -422,95 +464,90 @@ __global__ __launch_bounds__(64 * W) void rec_backward_kernel(Rows<const T> dh, 
                 e[v] = a[j][v] * dv;
                 f[j][v] *= e[v];
             }
-        if (fr.all && at.whole) {
-#pragma unroll
-            for (int j = 0; j < R; ++j) {
-                store_vec<V>(dx.at(at.b, fr.s(j)) + at.c, d[j]);
-                store_vec<V>(dgate.at(at.b, fr.s(j)) + at.c, f[j]);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < R; ++j)
-                if (fr.t + j < t1) {
-#pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        d[j][v] = fr.live(j) ? d[j][v] : 0.f;
-                        f[j][v] = fr.live(j) ? f[j][v] : 0.f;
-                    }
-                    rec_store<V>(dx.at(at.b, fr.s(j)) + at.c, at.own, d[j]);
-                    rec_store<V>(dgate.at(at.b, fr.s(j)) + at.c, at.own, f[j]);
-                }
-        }
+        dx.store(fr, at.whole, at.own, d);
+        dgate.store(fr, at.whole, at.own, f);
     }
-    if (dh0 && t0 == 0 && at.wave == 0 && at.tl == 0) rec_store<V>(dh0 + (long)at.b * C + at.c, at.own, carry);
+    if (dh0 && t0 == 0 && at.first()) rec_store<V>(dh0 + (long)at.b * C + at.c, at.own, carry);
 }
 
-constexpr int REC_V = 2;                                       // channels a lane
-constexpr int rec_rows(int bytes, bool backward) { return backward || bytes == 4 ? 8 : 16; }     // frames a thread
+constexpr int REC_V = 2, REC_R = 8;                            // channels and frames a thread
+// the short form's waves: as many as reach from one saved state to the next
+constexpr int rec_short(int lanes) { return std::max(1, REC_SAVE / (64 / lanes * REC_R)); }
 
-// `rows` frames a thread; slices of REC_LC V channels; pieces until the chip is filled.
-static inline RecPlan rec_plan(int B, int S, int C, int rows) {
+// Slices of 256 bytes of a frame where that leaves a workgroup for every CU, else of 128: two lines a row reach 4.9 TB/s, one 4.3
+// (64 x 3999 x 512 bf16 forward: 162 and 184 us).  A sequence is cut into pieces, each read twice, where whole sequences occupy less than
+// 192 of the 256 CUs; then into as many as stay on the chip at once, two workgroups a CU.
+static inline RecPlan rec_plan(int B, int S, int C, int bytes) {
     const int V = C >= REC_V ? REC_V : 1;
     RecPlan pl;
-    pl.slices = (C + REC_LC * V - 1) / (REC_LC * V);
-    pl.waves = S <= REC_LT * rows ? 1 : REC_WIDE;
-    const long tile = (long)pl.waves * REC_LT * rows, tiles = (S + tile - 1) / tile, seqs = (long)B * pl.slices;
-    const long want = seqs >= 192 ? 1 : std::min((512 + seqs - 1) / seqs, 64l);
-    const long per = std::max(1l, tiles / std::min(want, tiles));
-    pl.piece = per * tile;
+    pl.lanes = 128 / bytes;
+    if (V == 1 || (long)B * ((C + pl.lanes * V - 1) / (pl.lanes * V)) < 256) pl.lanes /= 2;
+    const int wave = 64 / pl.lanes * REC_R, few = rec_short(pl.lanes);
+    pl.slices = (C + pl.lanes * V - 1) / (pl.lanes * V);
+    pl.waves = S <= few * wave ? few : REC_WIDE;
+    const long tile = (long)pl.waves * wave, tiles = (S + tile - 1) / tile, seqs = (long)B * pl.slices;
+    const long want = seqs >= 192 ? 1 : std::min(512 / seqs, tiles);
+    const long per = (tiles + want - 1) / want;
+    pl.piece = (int)(per * tile);
     pl.pieces = (int)((tiles + per - 1) / per);
+    pl.near = true;
     return pl;
 }
-static inline size_t rec_ws_bytes(int B, int S, int C, int bytes, bool backward) {
-    const RecPlan pl = rec_plan(B, S, C, rec_rows(bytes, backward));
+static inline size_t rec_ws_bytes(int B, int S, int C, int bytes) {
+    const RecPlan pl = rec_plan(B, S, C, bytes);
     return pl.pieces == 1 ? 0 : align_up((size_t)B * pl.pieces * 2 * C * sizeof(float)) + align_up((size_t)B * C * sizeof(float));
 }
 
-// f(V, W) as integral constants
-template <class F> static int rec_shape(int C, const RecPlan& pl, F f) {
-    std::integral_constant<int, REC_V> v;
-    std::integral_constant<int, 1> one;
-    std::integral_constant<int, REC_WIDE> wide;
-    if (C >= REC_V) return pl.waves == 1 ? f(v, one) : f(v, wide);
-    return pl.waves == 1 ? f(one, one) : f(one, wide);
+// f(RecShape) of the form that the plan names
+template <class T, int V, int LC, class F> static int rec_waves(const RecPlan& pl, F f) {
+    return pl.waves == REC_WIDE ? f(RecShape<T, V, LC, REC_R, REC_WIDE>()) : f(RecShape<T, V, LC, REC_R, rec_short(LC)>());
+}
+template <class T, class F> static int rec_shape(int C, const RecPlan& pl, F f) {
+    constexpr int LC = 128 / sizeof(T);
+    if (C < REC_V) return rec_waves<T, 1, LC / 2>(pl, f);
+    return pl.lanes == LC ? rec_waves<T, REC_V, LC>(pl, f) : rec_waves<T, REC_V, LC / 2>(pl, f);
+}
+// whether a tile of an operand can be addressed by 32-bit offsets
+template <class Q, class U> static bool rec_near(const Rows<U>& r, int C) {
+    return r.row >= 0 && r.row < (1l << 31) / (Q::TILE * (long)sizeof(U)) && C < 1 << 28;
 }
 
 template <class T>
 static int run_recurrence(Rows<const T> x, Rows<const T> gate, const float* h0, const int* lengths, Rows<T> h, float* last, float* saved,
-                          int B, int S, int C, int reverse, void* ws, hipStream_t st) {
-    constexpr int R = rec_rows(sizeof(T), false);
-    const RecPlan pl = rec_plan(B, S, C, R);
+                          int B, int S, int C, bool reverse, void* ws, hipStream_t st) {
+    RecPlan pl = rec_plan(B, S, C, sizeof(T));
     Arena arena(ws, ~(size_t)0);
     float* agg = pl.pieces > 1 ? arena.take<float>((size_t)B * pl.pieces * 2 * C) : nullptr;
     float* kept = pl.pieces > 1 ? arena.take<float>((size_t)B * C) : nullptr;
     const long grid = (long)B * pl.pieces * pl.slices;
     if (grid > 0x7fffffff) return MSF2_ERR_ARG;
-    return rec_shape(C, pl, [&](auto v, auto w) {
-        constexpr int V = decltype(v)::value, W = decltype(w)::value;
-        if constexpr (W > 1)
-            if (pl.pieces > 1) rec_piece_kernel<false, T, V, W><<<grid, 64 * W, 0, st>>>(x, gate, h0, lengths, agg, kept, pl, S, C, reverse);
-        rec_forward_kernel<T, V, R, W><<<grid, 64 * W, 0, st>>>(x, gate, pl.pieces > 1 ? kept : h0, lengths, h, last, saved, agg, pl, S, C, reverse);
+    return rec_shape<T>(C, pl, [&](auto q) {
+        typedef decltype(q) Q;
+        pl.near = rec_near<Q>(x, C) && rec_near<Q>(gate, C) && rec_near<Q>(h, C);
+        if constexpr (Q::W == REC_WIDE)
+            if (pl.pieces > 1) rec_piece_kernel<false, Q><<<grid, 64 * Q::W, 0, st>>>(x, gate, h0, lengths, agg, kept, pl, S, C, reverse);
+        rec_forward_kernel<Q><<<grid, 64 * Q::W, 0, st>>>(x, gate, pl.pieces > 1 ? kept : h0, lengths, h, last, saved, agg, pl, S, C, reverse);
         return check_launch();
     });
 }
 
 template <class T>
 static int run_recurrence_backward(Rows<const T> dh, Rows<const T> x, Rows<const T> gate, const float* saved, const float* dlast,
-                                   const int* lengths, Rows<T> dx, Rows<T> dgate, float* dh0, int B, int S, int C, int reverse, void* ws,
+                                   const int* lengths, Rows<T> dx, Rows<T> dgate, float* dh0, int B, int S, int C, bool reverse, void* ws,
                                    hipStream_t st) {
-    constexpr int R = rec_rows(sizeof(T), true);
-    const RecPlan pl = rec_plan(B, S, C, R);
+    RecPlan pl = rec_plan(B, S, C, sizeof(T));
     Arena arena(ws, ~(size_t)0);
     float* agg = pl.pieces > 1 ? arena.take<float>((size_t)B * pl.pieces * 2 * C) : nullptr;
     float* kept = pl.pieces > 1 ? arena.take<float>((size_t)B * C) : nullptr;
     const long grid = (long)B * pl.pieces * pl.slices;
     if (grid > 0x7fffffff) return MSF2_ERR_ARG;
-    return rec_shape(C, pl, [&](auto v, auto w) {
-        constexpr int V = decltype(v)::value, W = decltype(w)::value;
-        if constexpr (W > 1)
-            if (pl.pieces > 1) rec_piece_kernel<true, T, V, W><<<grid, 64 * W, 0, st>>>(dh, gate, dlast, lengths, agg, kept, pl, S, C, reverse);
-        rec_backward_kernel<T, V, R, W><<<grid, 64 * W, 0, st>>>(dh, x, gate, saved, pl.pieces > 1 ? kept : dlast, lengths, dx, dgate, dh0, agg,
-                                                                 pl, S, C, reverse);
+    return rec_shape<T>(C, pl, [&](auto q) {
+        typedef decltype(q) Q;
+        pl.near = rec_near<Q>(dh, C) && rec_near<Q>(x, C) && rec_near<Q>(gate, C) && rec_near<Q>(dx, C) && rec_near<Q>(dgate, C);
+        if constexpr (Q::W == REC_WIDE)
+            if (pl.pieces > 1) rec_piece_kernel<true, Q><<<grid, 64 * Q::W, 0, st>>>(dh, gate, dlast, lengths, agg, kept, pl, S, C, reverse);
+        rec_backward_kernel<Q><<<grid, 64 * Q::W, 0, st>>>(dh, x, gate, saved, pl.pieces > 1 ? kept : dlast, lengths, dx, dgate, dh0, agg,
+                                                           pl, S, C, reverse);
         return check_launch();
     });
 }

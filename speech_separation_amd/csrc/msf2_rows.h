@@ -41,11 +41,13 @@ template <int V, class T> __device__ __forceinline__ typename VecOf<T, V>::type 
         if (j < n) v[j] = p[j];
     return v;
 }
-template <int V, class T> __device__ __forceinline__ void store_vec(T* p, const float (&f)[V]) {
+// PAST: past the caches, for results that would only push the operands out of them.
+template <int V, bool PAST = false, class T> __device__ __forceinline__ void store_vec(T* p, const float (&f)[V]) {
     typename VecOf<T, V>::type v;
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = (T)f[j];
-    *reinterpret_cast<typename VecOf<T, V>::type*>(p) = v;
+    if constexpr (PAST) __builtin_nontemporal_store(v, reinterpret_cast<typename VecOf<T, V>::type*>(p));
+    else *reinterpret_cast<typename VecOf<T, V>::type*>(p) = v;
 }
 template <int V, class T> __device__ __forceinline__ void store_some(T* p, int n, const float (&f)[V]) {
 #pragma unroll
@@ -69,35 +71,40 @@ __device__ __forceinline__ int frames_of(const int* lengths, int b, int S) {
     return lengths ? min(max(lengths[b], 0), S) : S;
 }
 
-// 1 / (1 + e^-v) and its complement 1 / (1 + e^v) without cancellation: the exponential of -|v| only, so neither overflows.
-// e^-|v| = 2^t (1 + r), t = -|v| log2 e rounded and r the part of the product that the rounding and the constant's own tail
-// leave out: v_exp_f32 alone would carry |v| half-steps of error into a gate near 0 or 1.
-__device__ __forceinline__ void sigmoid_pair(float v, float& p, float& q) {
-    const float n = -fabsf(v), t = n * 1.44269504088896f;
-    const float r = fmaf(n, 1.44269504088896f, -t) + n * 1.925963033e-8f;
-    float e = __builtin_amdgcn_exp2f(t);
-    e = fmaf(e, 0.693147180559945f * (t < -126.f ? 0.f : r), e);        // -infinity: t is, and r is not a number
-    const float d = __builtin_amdgcn_rcpf(1.f + e), s = e * d;
-    p = v < 0.f ? s : d;
-    q = v < 0.f ? d : s;
+// p = 1 / (1 + t) and q = 1 - p = t p, t = e^-v: neither cancels.  A rounding d of v log2 e is a relative error d ln 2 of t, which p takes
+// q times and q takes p times: FINE (fp32 operands) adds the part that the product's rounding left out.  Values beyond 87 are
+// held there (e^87 and its inverse are normal numbers; maximum and minimum keep NaN).
+template <bool FINE> __device__ __forceinline__ void sigmoid_pair(float v, float& p, float& q) {
+    constexpr float LOG2E = 1.44269504088896f, LN2 = 0.693147180559945f;
+    v = __builtin_elementwise_maximum(v, -87.f);
+    if constexpr (FINE) v = __builtin_elementwise_minimum(v, 87.f);
+    const float u = -v * LOG2E;
+    float t = __builtin_amdgcn_exp2f(u);
+    if constexpr (FINE) t = fmaf(t * LN2, fmaf(-v, LOG2E, -u), t);
+    p = __builtin_amdgcn_rcpf(1.f + t);
+    q = t * p;
 }
+template <class T> constexpr bool fine() { return sizeof(T) == 4; }
 
-template <int ACT> __device__ __forceinline__ float act_f(float v) {
+// v p of minus infinity is 0, not a product of infinity and the least p
+__device__ __forceinline__ float silu_of(float v, float p) { return __builtin_elementwise_maximum(v, -87.f) * p; }
+
+template <int ACT, bool FINE> __device__ __forceinline__ float act_f(float v) {
     if constexpr (ACT == MSF2_ACT_RELU) return v < 0.f ? 0.f : v;       // keeps NaN
     if constexpr (ACT == MSF2_ACT_SILU || ACT == MSF2_ACT_SIGMOID) {
         float p, q;
-        sigmoid_pair(v, p, q);
-        return ACT == MSF2_ACT_SILU ? v * p : p;
+        sigmoid_pair<FINE>(v, p, q);
+        return ACT == MSF2_ACT_SILU ? silu_of(v, p) : p;
     }
     return v;
 }
 // act'(v)
-template <int ACT> __device__ __forceinline__ float act_grad_f(float v) {
+template <int ACT, bool FINE> __device__ __forceinline__ float act_grad_f(float v) {
     if constexpr (ACT == MSF2_ACT_RELU) return v > 0.f ? 1.f : 0.f;
     if constexpr (ACT == MSF2_ACT_SILU || ACT == MSF2_ACT_SIGMOID) {
         float p, q;
-        sigmoid_pair(v, p, q);
-        return ACT == MSF2_ACT_SILU ? p * fmaf(v, q, 1.f) : p * q;
+        sigmoid_pair<FINE>(v, p, q);
+        return ACT == MSF2_ACT_SILU ? p * fmaf(__builtin_elementwise_minimum(__builtin_elementwise_maximum(v, -87.f), 87.f), q, 1.f) : p * q;
     }
     return 1.f;
 }
