@@ -59,11 +59,11 @@ template <int V, class T> __device__ __forceinline__ void store_some(T* p, int n
 // n m / 2^(31+l) is off by less than 1 / d and its whole part is right.
 struct Divider {
     unsigned d, m, shift;
-    explicit Divider(unsigned d_) : d(d_), shift(31) {
+    explicit Divider(unsigned d_ = 1) : d(d_), shift(31) {
         while ((1ull << (shift - 31)) < d) ++shift;
         m = (unsigned)((1ull << shift) / d + 1);
     }
-    __device__ __forceinline__ unsigned div(unsigned n) const { return (unsigned)((uint64_t)n * m >> shift); }
+    __host__ __device__ __forceinline__ unsigned div(unsigned n) const { return (unsigned)((uint64_t)n * m >> shift); }
 };
 
 // Frames of utterance b: lengths[b] held to [0, S], all S without lengths.
