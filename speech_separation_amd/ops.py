@@ -174,6 +174,10 @@ def gated_fsmn(x, packed):
     return y
 
 
+# The current stream's handle without the Python object around it: 2 us less in a call that takes about 10.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 # ---- operators of a gated recurrent block: group norm with an activation, gated recurrence, dropout ------------------
 # Plain functions: they record nothing for autograd (speech_separation_amd.autograd does) and they may be captured into a
 # HIP graph, workspaces included, which come from torch's allocator for every call.
@@ -243,9 +247,11 @@ def _call(name, dev, ws_bytes, args):
         with torch.cuda.device(dev):
             return _call(name, dev, ws_bytes, args)
     if ws_bytes is not None:
-        ws = _ws(ws_bytes, dev)
-        args = (*args, ws.data_ptr(), ws.numel())
-    _lib.check(getattr(_lib.load(), name)(*args, torch.cuda.current_stream(dev).cuda_stream), name)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+        args = (*args, ws.data_ptr() if ws_bytes else None, ws_bytes)
+    rc = getattr(_lib.load(), name)(*args, _raw_stream(dev.index))
+    if rc:
+        _lib.check(rc, name)
 
 
 def group_norm_act(x, gamma, beta, groups, eps=1e-5, act=_lib.ACT_NONE, act_first=False, lengths=None):
