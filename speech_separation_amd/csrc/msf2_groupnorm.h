@@ -17,30 +17,34 @@
 
 namespace msf2 {
 
-constexpr int GN_T = 256;                    // threads of a workgroup
+constexpr int GN_T = 512;                    // most threads of a workgroup
+constexpr int GN_LANES = 128;                // most lanes over the channels of a frame
 constexpr int GN_ROWS = 64;                  // frames a thread sums in 32 bits at most
 
-// Division of the work: `slices` of `width` channels (64 lanes x V, fewer lanes where C is narrow) by `chunks` of `rows` frames by
-// utterances.  Within a slice a group counts from the first that touches it; at most `local` groups do.
+// Division of the work: `slices` of `width` channels (`lanes` x V) by `chunks` of `rows` frames by utterances.  Within a slice a group counts from the first that touches it; at most `local` groups do.
 struct GnPlan {
-    int lanes, width, slices, chunks, rows, local, D;
+    int lanes, step, threads, width, slices, chunks, rows, local, D;     // step: frames that a workgroup takes side by side
     Divider by_D, by_width;
     __device__ int group(int c) const { return by_D.div(c); }
     __device__ int first(int slice) const { return group(slice * width); }
     __device__ int last(int slice, int C) const { return group(min((slice + 1) * width, C) - 1); }
 };
 
+// A thread's place.  The lane of the last channels is moved left to end with the row, so that every access is a whole vector: what
+// it shares with its neighbour (below `own`) counts for nothing in sums and is stored twice with the same value.
 template <int V> struct GnPlace {
-    int b, slice, chunk, c, r0, step, have;
+    int b, slice, chunk, c, r0, step, have, own;
     __device__ GnPlace(const GnPlan& pl, unsigned block, int C) {
         slice = block % pl.slices;
         const unsigned rest = block / pl.slices;
         chunk = rest % pl.chunks;
         b = rest / pl.chunks;
-        c = slice * pl.width + threadIdx.x % pl.lanes * V;
-        have = min(C - c, V);                // channels of this lane, none or less past the row's end
         r0 = threadIdx.x / pl.lanes;
-        step = GN_T / pl.lanes;
+        c = slice * pl.width + (threadIdx.x - r0 * pl.lanes) * V;
+        step = pl.step;
+        have = r0 < step ? min(C - c, V) : 0;        // channels of this lane, none or less past the row's end
+        own = C >= V && have > 0 ? V - have : 0;
+        c -= own;
     }
 };
 
@@ -49,14 +53,14 @@ struct Moments {
 };
 
 // V channels' values of a vector over channels (null: `none`), and of a pair of values per group.
-template <int V> __device__ __forceinline__ void gn_channels(const float* p, int c, int have, float none, float (&f)[V]) {
-    if (p && have >= V) {
+template <int V> __device__ __forceinline__ void gn_channels(const float* p, int c, int C, float none, float (&f)[V]) {
+    if (p && c + V <= C) {
         const auto u = load_vec<V>(p + c);
 #pragma unroll
         for (int v = 0; v < V; ++v) f[v] = u[v];
     } else {
 #pragma unroll
-        for (int v = 0; v < V; ++v) f[v] = p && v < have ? p[c + v] : none;
+        for (int v = 0; v < V; ++v) f[v] = p && c + v < C ? p[c + v] : none;
     }
 }
 template <int V> __device__ __forceinline__ void gn_of_groups(const float* pairs, const GnPlan& pl, int c, int C, float (&a)[V], float (&b)[V]) {
@@ -74,13 +78,21 @@ template <int V> __device__ __forceinline__ void gn_of_groups(const float* pairs
     }
 }
 
-// One vector of a frame: whole, or the last channels of the row.
-template <int V, class T> __device__ __forceinline__ typename VecOf<T, V>::type gn_load(const T* p, int have) {
-    return have >= V ? load_vec<V>(p) : load_some<V>(p, have);
+// One vector of a frame.  C < V, the same for the whole launch: frames narrower than a vector.
+template <int V, class T> __device__ __forceinline__ typename VecOf<T, V>::type gn_load(const T* p, int C) {
+    return C >= V ? load_vec<V>(p) : load_some<V>(p, C);
 }
-template <int V, class T> __device__ __forceinline__ void gn_store(T* p, int have, const float (&f)[V]) {
-    if (have >= V) store_vec<V, true>(p, f);
-    else store_some<V>(p, have, f);
+template <int V, class T> __device__ __forceinline__ void gn_store(T* p, int C, const float (&f)[V]) {
+    if (C >= V) store_vec<V, true>(p, f);
+    else store_some<V>(p, C, f);
+}
+// this thread's own channels into its row of a table [step][width]
+template <int V> __device__ __forceinline__ void gn_note(float* table, const GnPlan& pl, const GnPlace<V>& at, const float (&f)[V]) {
+    if (at.have <= 0) return;
+    float* p = table + at.r0 * pl.width + at.c - at.slice * pl.width;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+        if (v >= at.own) p[v] = f[v];
 }
 
 template <int J> __device__ __forceinline__ float sum_lanes(float v) {
@@ -95,8 +107,8 @@ template <int J> __device__ __forceinline__ double sum_lanes(double v) {
 }
 // f(J) with J threads a group: a wave where there are few
 template <class F> __device__ __forceinline__ void gn_spread(int groups, F f) {
-    if (groups <= GN_T / 64) f(std::integral_constant<int, 64>());
-    else if (groups <= GN_T / 32) f(std::integral_constant<int, 32>());
+    if (groups <= (int)blockDim.x / 64) f(std::integral_constant<int, 64>());
+    else if (groups <= (int)blockDim.x / 32) f(std::integral_constant<int, 32>());
     else f(std::integral_constant<int, 16>());
 }
 
@@ -104,7 +116,7 @@ template <class F> __device__ __forceinline__ void gn_spread(int groups, F f) {
 // chunks and slices, a J-th of them a thread.
 template <int J, class P, class F> __device__ __forceinline__ void gn_groups(const P* part, const GnPlan& pl, int b, int slice, int C, F f) {
     const int g0 = pl.first(slice), groups = pl.last(slice, C) - g0 + 1, j = threadIdx.x % J;
-    for (int g = threadIdx.x / J; g < groups; g += GN_T / J) {
+    for (int g = threadIdx.x / J; g < groups; g += blockDim.x / J) {
         const int a = pl.by_width.div((g0 + g) * pl.D), z = pl.by_width.div((g0 + g + 1) * pl.D - 1);
         f(g, j, [&](auto h) {
             for (int sl = a; sl <= z; ++sl) {
@@ -129,13 +141,13 @@ __global__ __launch_bounds__(GN_T) void gn_moments_kernel(Rows<const T> x, const
     const bool some = at.have > 0 && s0 + at.r0 < s1;
     auto fetch = [&](int r) {
 #pragma unroll
-        for (int j = 0; j < U; ++j) u[j] = gn_load<V>(x.at(at.b, min(r + j * at.step, s1 - 1)) + at.c, at.have);
+        for (int j = 0; j < U; ++j) u[j] = gn_load<V>(x.at(at.b, min(r + j * at.step, s1 - 1)) + at.c, C);
     };
     float K[V], s[V], q[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) s[v] = q[v] = 0.f;
     if (some) {
-        k = gn_load<V>(x.at(at.b, s0) + at.c, at.have);
+        k = gn_load<V>(x.at(at.b, s0) + at.c, C);
         fetch(s0 + at.r0);
 #pragma unroll
         for (int v = 0; v < V; ++v) K[v] = act_f<PRE, fine<T>()>((float)k[v]);
@@ -156,13 +168,13 @@ __global__ __launch_bounds__(GN_T) void gn_moments_kernel(Rows<const T> x, const
             }
         }
     }
-#pragma unroll
-    for (int v = 0; v < V; ++v) s_s[threadIdx.x * V + v] = s[v], q_s[threadIdx.x * V + v] = q[v];
+    gn_note<V>(s_s, pl, at, s);
+    gn_note<V>(q_s, pl, at, q);
     __syncthreads();
     // a channel's frames together: (mean, M2) over the chunk; this thread alone reads and writes column i
     const int w = min(pl.width, C - c0);
     const float count = (float)max(s1 - s0, 0), inv = count > 0.f ? 1.f / count : 0.f;
-    for (int i = threadIdx.x; i < w; i += GN_T) {
+    for (int i = threadIdx.x; i < w; i += blockDim.x) {
         float p = 0.f, m = 0.f;
         for (int k = 0; k < at.step; ++k) p += s_s[k * pl.width + i], m += q_s[k * pl.width + i];
         const float first = count > 0.f ? act_f<PRE, fine<T>()>((float)x.at(at.b, s0)[c0 + i]) : 0.f;
@@ -175,7 +187,7 @@ __global__ __launch_bounds__(GN_T) void gn_moments_kernel(Rows<const T> x, const
     gn_spread(groups, [&](auto jj) {
         constexpr int J = decltype(jj)::value;
         const int j = threadIdx.x % J;
-        for (int g = threadIdx.x / J; g < groups; g += GN_T / J) {
+        for (int g = threadIdx.x / J; g < groups; g += blockDim.x / J) {
             const int w0 = max((g0 + g) * pl.D - c0, 0), w1 = min((g0 + g + 1) * pl.D - c0, w);
             float mean = 0.f, m2 = 0.f;
             for (int i = w0 + j; i < w1; i += J) mean += s_s[i];
@@ -223,7 +235,7 @@ __global__ __launch_bounds__(GN_T) void gn_apply_kernel(Rows<const T> x, const f
     auto fetch = [&](int r) {
         if (at.have > 0) {
 #pragma unroll
-            for (int j = 0; j < U; ++j) u[j] = gn_load<V>(x.at(at.b, min(r + j * at.step, min(s1 - 1, cap))) + at.c, at.have);
+            for (int j = 0; j < U; ++j) u[j] = gn_load<V>(x.at(at.b, min(r + j * at.step, min(s1 - 1, cap))) + at.c, C);
         }
     };
     fetch(s0 + at.r0);                       // on its way while the sums are joined
@@ -231,12 +243,12 @@ __global__ __launch_bounds__(GN_T) void gn_apply_kernel(Rows<const T> x, const f
     gn_join_moments(part, pl, at.b, at.slice, C, eps, st);
     __syncthreads();
     if (at.chunk == 0)                       // slices that share a group write the same values
-        for (int i = threadIdx.x; i < 2 * groups; i += GN_T) stats[2 * ((long)at.b * G + g0) + i] = st[i];
+        for (int i = threadIdx.x; i < 2 * groups; i += blockDim.x) stats[2 * ((long)at.b * G + g0) + i] = st[i];
     if (at.have <= 0) return;
     float mean[V], ga[V], be[V], rstd[V];
     gn_of_groups<V>(st - 2 * g0, pl, at.c, C, mean, rstd);
-    gn_channels<V>(gamma, at.c, at.have, 1.f, ga);
-    gn_channels<V>(beta, at.c, at.have, 0.f, be);
+    gn_channels<V>(gamma, at.c, C, 1.f, ga);
+    gn_channels<V>(beta, at.c, C, 0.f, be);
 #pragma unroll
     for (int v = 0; v < V; ++v) ga[v] *= rstd[v];
     for (int r = s0 + at.r0; r < s1; r += U * at.step) {
@@ -254,7 +266,7 @@ __global__ __launch_bounds__(GN_T) void gn_apply_kernel(Rows<const T> x, const f
                 f[v] = act_f<POST, fine<T>()>(fmaf(act_f<PRE, fine<T>()>((float)w[j][v]) - mean[v], ga[v], be[v]));
                 if (s >= n) f[v] = 0.f;
             }
-            gn_store<V>(y.at(at.b, s) + at.c, at.have, f);
+            gn_store<V>(y.at(at.b, s) + at.c, C, f);
         }
     }
 }
@@ -275,16 +287,16 @@ __global__ __launch_bounds__(GN_T) void gn_grad_sums_kernel(Rows<const T> dy, Ro
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             const int s = min(r + j * at.step, s1 - 1);
-            u[j] = gn_load<V>(x.at(at.b, s) + at.c, at.have);
-            d[j] = gn_load<V>(dy.at(at.b, s) + at.c, at.have);
+            u[j] = gn_load<V>(x.at(at.b, s) + at.c, C);
+            d[j] = gn_load<V>(dy.at(at.b, s) + at.c, C);
         }
     };
     const bool some = at.have > 0 && s0 + at.r0 < s1;
     if (some) fetch(s0 + at.r0);
     float mean[V], rstd[V], ga[V], be[V], a1[V], a2[V];
     gn_of_groups<V>(stats + 2 * (long)at.b * G, pl, at.c, C, mean, rstd);
-    gn_channels<V>(gamma, at.c, at.have, 1.f, ga);
-    gn_channels<V>(beta, at.c, at.have, 0.f, be);
+    gn_channels<V>(gamma, at.c, C, 1.f, ga);
+    gn_channels<V>(beta, at.c, C, 0.f, be);
 #pragma unroll
     for (int v = 0; v < V; ++v) a1[v] = a2[v] = 0.f;
     if (some)
@@ -305,15 +317,12 @@ __global__ __launch_bounds__(GN_T) void gn_grad_sums_kernel(Rows<const T> dy, Ro
                 }
             }
         }
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        s1_s[threadIdx.x * V + v] = a1[v];
-        s2_s[threadIdx.x * V + v] = a2[v];
-    }
+    gn_note<V>(s1_s, pl, at, a1);
+    gn_note<V>(s2_s, pl, at, a2);
     __syncthreads();
     const int w = min(pl.width, C - c0);
     float* out = chan + ((long)at.b * pl.chunks + at.chunk) * 2 * C + c0;
-    for (int i = threadIdx.x; i < w; i += GN_T) {
+    for (int i = threadIdx.x; i < w; i += blockDim.x) {
         float p = 0.f, q = 0.f;
         for (int k = 0; k < at.step; ++k) p += s1_s[k * pl.width + i], q += s2_s[k * pl.width + i];
         out[i] = p;
@@ -327,7 +336,7 @@ __global__ __launch_bounds__(GN_T) void gn_grad_sums_kernel(Rows<const T> dy, Ro
     gn_spread(groups, [&](auto jj) {
         constexpr int J = decltype(jj)::value;
         const int j = threadIdx.x % J;
-        for (int g = threadIdx.x / J; g < groups; g += GN_T / J) {
+        for (int g = threadIdx.x / J; g < groups; g += blockDim.x / J) {
             const int w0 = max((g0 + g) * pl.D - c0, 0), w1 = min((g0 + g + 1) * pl.D - c0, w);
             float p = 0.f, q = 0.f;
             for (int i = w0 + j; i < w1; i += J) p += s1_s[i], q += s2_s[i];
@@ -341,9 +350,8 @@ __global__ __launch_bounds__(GN_T) void gn_grad_sums_kernel(Rows<const T> dy, Ro
 constexpr int GN_SUM_C = 16;                 // channels of a workgroup that adds up dgamma and dbeta
 // dgamma and dbeta of 16 channels over utterances and chunks, in 64 bits
 __device__ __forceinline__ void gn_gain_sums(const float* chan, float* dgamma, float* dbeta, long parts, int C, unsigned block) {
-    constexpr int K = GN_T / GN_SUM_C;
-    __shared__ double red[2][K][GN_SUM_C];
-    const int i = threadIdx.x % GN_SUM_C, k = threadIdx.x / GN_SUM_C, c = block * GN_SUM_C + i;
+    __shared__ double red[2][GN_T / GN_SUM_C][GN_SUM_C];
+    const int K = blockDim.x / GN_SUM_C, i = threadIdx.x % GN_SUM_C, k = threadIdx.x / GN_SUM_C, c = block * GN_SUM_C + i;
     double p = 0, q = 0;
     if (c < C) {
 #pragma unroll 8
@@ -380,8 +388,8 @@ __global__ __launch_bounds__(GN_T) void gn_dx_kernel(Rows<const T> dy, Rows<cons
 #pragma unroll
             for (int j = 0; j < U; ++j) {
                 const int s = min(r + j * at.step, min(s1 - 1, cap));
-                u[j] = gn_load<V>(x.at(at.b, s) + at.c, at.have);
-                d[j] = gn_load<V>(dy.at(at.b, s) + at.c, at.have);
+                u[j] = gn_load<V>(x.at(at.b, s) + at.c, C);
+                d[j] = gn_load<V>(dy.at(at.b, s) + at.c, C);
             }
         }
     };
@@ -402,8 +410,8 @@ __global__ __launch_bounds__(GN_T) void gn_dx_kernel(Rows<const T> dy, Rows<cons
     float mean[V], rstd[V], ga[V], be[V], c1[V], c2[V];
     gn_of_groups<V>(stats + 2 * (long)at.b * G, pl, at.c, C, mean, rstd);
     gn_of_groups<V>(st - 2 * g0, pl, at.c, C, c1, c2);
-    gn_channels<V>(gamma, at.c, at.have, 1.f, ga);
-    gn_channels<V>(beta, at.c, at.have, 0.f, be);
+    gn_channels<V>(gamma, at.c, C, 1.f, ga);
+    gn_channels<V>(beta, at.c, C, 0.f, be);
     for (int r = s0 + at.r0; r < s1; r += U * at.step) {
         typename VecOf<T, V>::type w[U], e[U];
 #pragma unroll
@@ -421,7 +429,7 @@ __global__ __launch_bounds__(GN_T) void gn_dx_kernel(Rows<const T> dy, Rows<cons
                 f[v] = rstd[v] * (fmaf(dz, ga[v], -c1[v]) - xh * c2[v]) * act_grad_f<PRE, fine<T>()>(xv);
                 if (s >= n) f[v] = 0.f;
             }
-            gn_store<V>(dx.at(at.b, s) + at.c, at.have, f);
+            gn_store<V>(dx.at(at.b, s) + at.c, C, f);
         }
     }
 }
@@ -433,16 +441,21 @@ static inline GnPlan gn_plan(int B, int S, int C, int G, int bytes) {
     const int V = gn_vec(bytes), vecs = (C + V - 1) / V;
     pl.D = C / G;
     pl.by_D = Divider(pl.D);
-    pl.lanes = 1;
-    while (pl.lanes < 64 && pl.lanes < vecs) pl.lanes *= 2;
+    // Whole frames up to 128 lanes, so that a workgroup's frames are one piece of memory whatever their width; wider ones in equal slices.
+    // As many frames side by side as leave the fewest lanes of the waves idle, in 256 threads or 512.
+    const int cuts = (vecs + GN_LANES - 1) / GN_LANES;
+    pl.lanes = (vecs + cuts - 1) / cuts;
+    pl.step = 256 / pl.lanes;
+    auto idle = [&](int step) { const int t = step * pl.lanes; return 1. - (double)t / ((t + 63) / 64 * 64); };
+    if (idle(512 / pl.lanes) + 0.05 < idle(pl.step)) pl.step = 512 / pl.lanes;
+    pl.threads = (pl.step * pl.lanes + 63) / 64 * 64;
     pl.width = pl.lanes * V;
     pl.by_width = Divider(pl.width);
     pl.slices = (vecs + pl.lanes - 1) / pl.lanes;
     pl.local = std::min(G, (pl.width + pl.D - 2) / pl.D + 1);
-    // 4 workgroups a CU, each with 4 frames a thread at least
-    const int least = 4 * GN_T / pl.lanes;
-    const long want = std::max(1l, 1024 / ((long)B * pl.slices));
-    pl.rows = (int)std::min<long>(std::max<long>(least, (S + want - 1) / want), GN_ROWS * GN_T / pl.lanes);
+    // 4 frames a thread at least, 1024 threads a CU
+    const long want = std::max(1l, 1024 * 256 / pl.threads / ((long)B * pl.slices));
+    pl.rows = (int)std::min<long>(std::max<long>(4 * pl.step, (S + want - 1) / want), (long)GN_ROWS * pl.step);
     pl.chunks = (S + pl.rows - 1) / pl.rows;
     return pl;
 }
@@ -459,8 +472,8 @@ static int run_group_norm(Rows<const T> x, const float* gamma, const float* beta
     const GnPlan pl = gn_plan(B, S, C, G, sizeof(T));
     const long grid = (long)B * pl.chunks * pl.slices;
     if (grid > 0x7fffffff) return MSF2_ERR_ARG;
-    gn_moments_kernel<T, V, PRE><<<grid, GN_T, 0, st>>>(x, lengths, (Moments*)ws, pl, S, C);
-    gn_apply_kernel<T, V, PRE, POST><<<grid, GN_T, pl.local * 2 * sizeof(float), st>>>(x, gamma, beta, lengths, (const Moments*)ws, y, stats, eps, pl, S, C, G);
+    gn_moments_kernel<T, V, PRE><<<grid, pl.threads, 0, st>>>(x, lengths, (Moments*)ws, pl, S, C);
+    gn_apply_kernel<T, V, PRE, POST><<<grid, pl.threads, pl.local * 2 * sizeof(float), st>>>(x, gamma, beta, lengths, (const Moments*)ws, y, stats, eps, pl, S, C, G);
     return check_launch();
 }
 
@@ -474,8 +487,8 @@ static int run_group_norm_backward(Rows<const T> dy, Rows<const T> x, const floa
     if (grid + gains > 0x7fffffff) return MSF2_ERR_ARG;
     float2* part = (float2*)ws;
     float* chan = (float*)((char*)ws + gn_part_bytes(pl, B, sizeof(float2)));
-    gn_grad_sums_kernel<T, V, PRE, POST><<<grid, GN_T, 0, st>>>(dy, x, gamma, beta, stats, lengths, chan, part, pl, S, C, G);
-    gn_dx_kernel<T, V, PRE, POST><<<grid + gains, GN_T, pl.local * 2 * sizeof(float), st>>>(dy, x, gamma, beta, stats, lengths, chan, part, dx, dgamma,
+    gn_grad_sums_kernel<T, V, PRE, POST><<<grid, pl.threads, 0, st>>>(dy, x, gamma, beta, stats, lengths, chan, part, pl, S, C, G);
+    gn_dx_kernel<T, V, PRE, POST><<<grid + gains, pl.threads, pl.local * 2 * sizeof(float), st>>>(dy, x, gamma, beta, stats, lengths, chan, part, dx, dgamma,
                                                                                           dbeta, pl, (unsigned)gains, B, S, C, G);
     return check_launch();
 }

@@ -236,7 +236,7 @@ template <class Q, class U> struct RecRows {
         }
     }
     __device__ __forceinline__ void store(const RecFrames<Q>& fr, bool whole, int own, float (&f)[Q::R][Q::V]) const {
-        if (fr.all && whole) {
+        if (fr.all && (whole || own <= 0)) {
 #pragma unroll
             for (int j = 0; j < Q::R; ++j) store_vec<Q::V, true>(off(base(fr, j), mine), f[j]);
         } else {
