@@ -20,8 +20,10 @@ __device__ __forceinline__ uint4 philox10(uint4 c, uint2 k) {
 // y = residual + x keep scale of `rows` frames (of utterance blockIdx.y where the operands' utterances do not follow one
 // another).  A thread takes U times 8 neighbouring channels of a frame, the 128 bits of one generator call: 16 bits an element, because the
 // generator's 20 wide multiplications (a quarter of the vector rate each) would otherwise bind the kernel before memory does.
-// All loads go out before the first of them.
-template <class TX, class TY, bool RES, int U>
+// All loads go out before the first of them.  The last, narrower block of a frame is loaded as the frame's last 8 channels, its
+// bits are moved up to them, and only its own channels are stored: loads without a branch (one here cost 5 % at widths that are
+// multiples of 8, and element by element it was 10 to 40 % at others).  TAIL: there is such a block.
+template <class TX, class TY, bool RES, bool TAIL, int U>
 __global__ __launch_bounds__(256) void dropout_kernel(Rows<const TX> x, Rows<const TY> res, Rows<TY> y, const int64_t* rng,
                                                       unsigned site, unsigned thr, float scale, Divider per, unsigned blocks,
                                                       long block0, long block_batch, int C) {
@@ -31,22 +33,34 @@ __global__ __launch_bounds__(256) void dropout_kernel(Rows<const TX> x, Rows<con
     typename VecOf<TX, 8>::type xv[U];
     typename VecOf<TY, 8>::type rv[U];
     unsigned row[U];
-    int c[U], n[U];
+    int c[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const unsigned i = min(i0 + u * 256u, blocks - 1);
         row[u] = per.div(i);
         c[u] = (int)(i - row[u] * per.d) * 8;
-        n[u] = i0 + u * 256u < blocks ? min(C - c[u], 8) : 0;
-        xv[u] = n[u] == 8 ? load_vec<8>(x.at(b, row[u]) + c[u]) : load_some<8>(x.at(b, row[u]) + c[u], n[u]);
-        if constexpr (RES) rv[u] = n[u] == 8 ? load_vec<8>(res.at(b, row[u]) + c[u]) : load_some<8>(res.at(b, row[u]) + c[u], n[u]);
+        if (!TAIL || C >= 8) {
+            const int at = TAIL ? min(c[u], C - 8) : c[u];
+            xv[u] = load_vec<8>(x.at(b, row[u]) + at);
+            if constexpr (RES) rv[u] = load_vec<8>(res.at(b, row[u]) + at);
+        } else {
+            xv[u] = load_some<8>(x.at(b, row[u]), C);
+            if constexpr (RES) rv[u] = load_some<8>(res.at(b, row[u]), C);
+        }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const uint64_t block = (uint64_t)(block0 + b * block_batch) + i0 + u * 256u;
         const uint4 r = philox10(make_uint4((unsigned)block, (unsigned)(block >> 32), (unsigned)step, site),
                                  make_uint2((unsigned)seed, (unsigned)(seed >> 32)));
-        const unsigned w[4] = {r.x, r.y, r.z, r.w};
+        unsigned w[4] = {r.x, r.y, r.z, r.w};
+        const bool last = TAIL && C >= 8 && c[u] > C - 8;
+        if (last)
+            for (int k = C % 8; k < 8; ++k) {        // 8 - C % 8 half-words up
+#pragma unroll
+                for (int j = 3; j > 0; --j) w[j] = w[j] << 16 | w[j - 1] >> 16;
+                w[0] <<= 16;
+            }
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -54,8 +68,11 @@ __global__ __launch_bounds__(256) void dropout_kernel(Rows<const TX> x, Rows<con
             v[j] = bits >= thr ? (float)xv[u][j] * scale : 0.f;
             if constexpr (RES) v[j] += (float)rv[u][j];
         }
-        if (n[u] == 8) store_vec<8>(y.at(b, row[u]) + c[u], v);
-        else store_some<8>(y.at(b, row[u]) + c[u], n[u], v);
+        if (i0 + u * 256u >= blocks) continue;
+        TY* out = y.at(b, row[u]);
+        if (TAIL && C < 8) store_some<8>(out, C, v);
+        else if (last) store_last<8>(out + C - 8, 8 - C % 8, v);
+        else store_vec<8>(out + c[u], v);
     }
 }
 
@@ -82,8 +99,14 @@ static int run_dropout(Rows<const TX> x, Rows<const TY> res, Rows<TY> y, const i
             const Rows<const TY> rr = {res.p ? res.at(b, r) : nullptr, res.batch, res.row};
             const Rows<TY> yr = {y.at(b, r), y.batch, y.row};
             const long block0 = (b * rows + r) * per;
-            if (res.p) dropout_kernel<TX, TY, true, U><<<grid, 256, 0, st>>>(xr, rr, yr, rng, site, thr, scale, by, blocks, block0, rows * per, C);
-            else dropout_kernel<TX, TY, false, U><<<grid, 256, 0, st>>>(xr, rr, yr, rng, site, thr, scale, by, blocks, block0, rows * per, C);
+            auto go = [&](auto has_res, auto tail) {
+                dropout_kernel<TX, TY, decltype(has_res)::value, decltype(tail)::value, U>
+                    <<<grid, 256, 0, st>>>(xr, rr, yr, rng, site, thr, scale, by, blocks, block0, rows * per, C);
+            };
+            const std::true_type yes;
+            const std::false_type no;
+            if (res.p) C % 8 ? go(yes, yes) : go(yes, no);
+            else C % 8 ? go(no, yes) : go(no, no);
         }
     return check_launch();
 }

@@ -54,6 +54,28 @@ template <int V, class T> __device__ __forceinline__ void store_some(T* p, int n
     for (int j = 0; j < V; ++j)
         if (j < n) p[j] = (T)f[j];
 }
+// All from element n on, n the same for all lanes that come here: one access for each bit of V - n, V / 2 elements last.
+template <int V, class T> __device__ __forceinline__ void store_last(T* p, int n, const float (&f)[V]) {
+    auto bit = [&](auto width) {
+        constexpr int W = decltype(width)::value;
+        if constexpr (W < V) {
+            if (n & W) {
+                float g[W];
+#pragma unroll
+                for (int j = 0; j < W; ++j) {
+                    g[j] = 0.f;
+#pragma unroll
+                    for (int o = W; o < V; o += 2 * W) g[j] = n == o ? f[o + j] : g[j];
+                }
+                store_vec<W>(p + n, g);
+                n += W;
+            }
+        }
+    };
+    bit(std::integral_constant<int, 1>());   // n is a multiple of 2 after this one, of 4 after the next
+    bit(std::integral_constant<int, 2>());
+    bit(std::integral_constant<int, 4>());
+}
 
 // n / d for n < 2^31 by one multiplication: with 2^(l-1) < d <= 2^l the factor m = 2^(31+l) / d + 1 is off by less than 1, so
 // n m / 2^(31+l) is off by less than 1 / d and its whole part is right.
