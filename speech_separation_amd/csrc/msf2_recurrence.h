@@ -476,7 +476,8 @@ constexpr int rec_short(int lanes) { return std::max(1, REC_SAVE / (64 / lanes *
 
 // Slices of 256 bytes of a frame where that leaves a workgroup for every CU, else of 128: two lines a row reach 4.9 TB/s, one 4.3
 // (64 x 3999 x 512 bf16 forward: 162 and 184 us).  A sequence is cut into pieces, each read twice, where whole sequences occupy less than
-// 192 of the 256 CUs; then into as many as stay on the chip at once, two workgroups a CU.
+// 192 of the 256 CUs; then into as many as stay on the chip at once, two workgroups a CU.  Two tiles in a row take less time than
+// another launch does (8.3 and 9.5 us at 4 x 512 x 256 fp32), three take more (10.8 and 9.6).
 static inline RecPlan rec_plan(int B, int S, int C, int bytes) {
     const int V = C >= REC_V ? REC_V : 1;
     RecPlan pl;
@@ -486,7 +487,7 @@ static inline RecPlan rec_plan(int B, int S, int C, int bytes) {
     pl.slices = (C + pl.lanes * V - 1) / (pl.lanes * V);
     pl.waves = S <= few * wave ? few : REC_WIDE;
     const long tile = (long)pl.waves * wave, tiles = (S + tile - 1) / tile, seqs = (long)B * pl.slices;
-    const long want = seqs >= 192 ? 1 : std::min(512 / seqs, tiles);
+    const long want = seqs >= 192 || tiles <= 2 ? 1 : std::min(512 / seqs, tiles);
     const long per = (tiles + want - 1) / want;
     pl.piece = (int)(per * tile);
     pl.pieces = (int)((tiles + per - 1) / per);
