@@ -66,7 +66,7 @@ int msf2_group_norm_act_backward(const void* dy, int64_t dy_batch, int64_t dy_ro
 }
 
 size_t msf2_gated_recurrence_ws_bytes(int B, int S, int C, int type) {
-    return sizes_ok(B, S, C) && type_ok(type) ? rec_ws_bytes(B, S, C, type_bytes(type)) : 0;
+    return sizes_ok(B, S, C) && type_ok(type) ? rec_ws_bytes(B, S, C, type_bytes(type), false) : 0;
 }
 
 int msf2_gated_recurrence(const void* x, int64_t x_batch, int64_t x_row, const void* gate, int64_t gate_batch,
@@ -84,7 +84,7 @@ int msf2_gated_recurrence(const void* x, int64_t x_batch, int64_t x_row, const v
 }
 
 size_t msf2_gated_recurrence_backward_ws_bytes(int B, int S, int C, int type) {
-    return sizes_ok(B, S, C) && type_ok(type) ? rec_ws_bytes(B, S, C, type_bytes(type)) : 0;
+    return sizes_ok(B, S, C) && type_ok(type) ? rec_ws_bytes(B, S, C, type_bytes(type), true) : 0;
 }
 
 int msf2_gated_recurrence_backward(const void* dh, int64_t dh_batch, int64_t dh_row, const void* x, int64_t x_batch,

@@ -22,6 +22,7 @@ constexpr int REC_WIDE = 8;                  // waves of a workgroup, where a se
 struct RecPlan {
     int lanes, slices, pieces, waves, piece;
     bool near;                               // a tile's rows span less than 2^32 bytes in every operand
+    bool past;                               // results go past the caches
 };
 
 // The lanes of a workgroup: LC side by side over V channels each, the LT = 64 / LC groups of a wave one after the other in time,
@@ -40,7 +41,6 @@ template <class T_, int V_, int LC_, int R_, int W_> struct RecShape {
 // to the 8 XCDs in turn, so block i of XCD k takes the i-th of the k-th eighth of the work.
 template <class Q> struct RecPlace {
     int b, p, n, tl, cl, wave, c, own;
-    bool whole;                              // no lane of the workgroup is past the row's end
     __device__ RecPlace(const RecPlan& pl, const int* lengths, int S, int C) {
         const unsigned each = gridDim.x / 8, more = gridDim.x % 8, xcd = blockIdx.x % 8;
         const unsigned id = xcd * each + min(xcd, more) + blockIdx.x / 8;
@@ -56,7 +56,6 @@ template <class Q> struct RecPlace {
         const int c0 = (slice * Q::LC + cl) * Q::V;
         c = min(c0, C - Q::V);
         own = c0 - c;                        // V and more: nothing is this lane's own
-        whole = (slice + 1) * Q::LC * Q::V <= C;
     }
     __device__ __forceinline__ bool first() const { return wave == 0 && tl == 0; }
 };
@@ -235,10 +234,24 @@ template <class Q, class U> struct RecRows {
             for (int j = 0; j < Q::R; ++j) v[j] = load_vec<Q::V>(p + (long)fr.held(j) * row + c);
         }
     }
-    __device__ __forceinline__ void store(const RecFrames<Q>& fr, bool whole, int own, float (&f)[Q::R][Q::V]) const {
-        if (fr.all && (whole || own <= 0)) {
+    __device__ __forceinline__ void store(const RecFrames<Q>& fr, bool past, int own, float (&f)[Q::R][Q::V]) const {
+        if (fr.all && own <= 0) {
+            if (past) {                      // the empty statements keep the compiler from making one of the two
+                asm volatile("");
 #pragma unroll
-            for (int j = 0; j < Q::R; ++j) store_vec<Q::V, true>(off(base(fr, j), mine), f[j]);
+                for (int j = 0; j < Q::R; ++j) store_vec<Q::V, true>(off(base(fr, j), mine), f[j]);
+                asm volatile("");
+            } else {
+#pragma unroll
+                for (int j = 0; j < Q::R; ++j) store_vec<Q::V>(off(base(fr, j), mine), f[j]);
+            }
+        } else if (fr.all) {
+#pragma unroll
+            for (int v = 1; v < Q::V; ++v)
+                if (v >= own) {
+#pragma unroll
+                    for (int j = 0; j < Q::R; ++j) off(base(fr, j), mine)[v] = (U)f[j][v];
+                }
         } else {
 #pragma unroll
             for (int j = 0; j < Q::R; ++j)
@@ -372,7 +385,7 @@ __global__ __launch_bounds__(64 * Q::W) void rec_forward_kernel(Rows<const typen
         for (int j = 0; j < R; ++j)
 #pragma unroll
             for (int v = 0; v < V; ++v) f[j][v] = hv[v] = fmaf(a[j][v], hv[v], f[j][v]);
-        h.store(fr, at.whole, at.own, f);
+        h.store(fr, pl.past, at.own, f);
     }
     if (last && t1 == S && at.first()) rec_store<V>(last + (long)at.b * C + at.c, at.own, carry);
 }
@@ -464,8 +477,8 @@ __global__ __launch_bounds__(64 * Q::W) void rec_backward_kernel(Rows<const type
                 e[v] = a[j][v] * dv;
                 f[j][v] *= e[v];
             }
-        dx.store(fr, at.whole, at.own, d);
-        dgate.store(fr, at.whole, at.own, f);
+        dx.store(fr, pl.past, at.own, d);
+        dgate.store(fr, pl.past, at.own, f);
     }
     if (dh0 && t0 == 0 && at.first()) rec_store<V>(dh0 + (long)at.b * C + at.c, at.own, carry);
 }
@@ -475,10 +488,12 @@ constexpr int REC_V = 2, REC_R = 8;                            // channels and f
 constexpr int rec_short(int lanes) { return std::max(1, REC_SAVE / (64 / lanes * REC_R)); }
 
 // Slices of 256 bytes of a frame where that leaves a workgroup for every CU, else of 128: two lines a row reach 4.9 TB/s, one 4.3
-// (64 x 3999 x 512 bf16 forward: 162 and 184 us).  A sequence is cut into pieces, each read twice, where whole sequences occupy less than
-// 192 of the 256 CUs; then into as many as stay on the chip at once, two workgroups a CU.  Two tiles in a row take less time than
-// another launch does (8.3 and 9.5 us at 4 x 512 x 256 fp32), three take more (10.8 and 9.6).
-static inline RecPlan rec_plan(int B, int S, int C, int bytes) {
+// (64 x 3999 x 512 bf16 forward: 162 and 184 us).  A sequence is cut into pieces, each read twice, where whole sequences occupy
+// less than 192 of the 256 CUs (16 x 4000 x 512 bf16 forward, 128 workgroups: 58 us in pieces, 74 whole); then into as many as stay
+// on the chip at once, two workgroups a CU forward and, for its registers, one backward (the same case: backward 81 us in 256
+// workgroups, 88 in 512; forward 64 and 58).  Two tiles in a row take less time than another launch does (8.3 and 9.5 us at 4 x 512 x 256
+// fp32), three take more (10.8 and 9.6).
+static inline RecPlan rec_plan(int B, int S, int C, int bytes, bool backward) {
     const int V = C >= REC_V ? REC_V : 1;
     RecPlan pl;
     pl.lanes = 128 / bytes;
@@ -487,15 +502,15 @@ static inline RecPlan rec_plan(int B, int S, int C, int bytes) {
     pl.slices = (C + pl.lanes * V - 1) / (pl.lanes * V);
     pl.waves = S <= few * wave ? few : REC_WIDE;
     const long tile = (long)pl.waves * wave, tiles = (S + tile - 1) / tile, seqs = (long)B * pl.slices;
-    const long want = seqs >= 192 || tiles <= 2 ? 1 : std::min(512 / seqs, tiles);
+    const long want = seqs >= 192 || tiles <= 2 ? 1 : std::min((backward ? 256 : 512) / seqs, tiles);
     const long per = (tiles + want - 1) / want;
     pl.piece = (int)(per * tile);
     pl.pieces = (int)((tiles + per - 1) / per);
-    pl.near = true;
+    pl.near = pl.past = true;
     return pl;
 }
-static inline size_t rec_ws_bytes(int B, int S, int C, int bytes) {
-    const RecPlan pl = rec_plan(B, S, C, bytes);
+static inline size_t rec_ws_bytes(int B, int S, int C, int bytes, bool backward) {
+    const RecPlan pl = rec_plan(B, S, C, bytes, backward);
     return pl.pieces == 1 ? 0 : align_up((size_t)B * pl.pieces * 2 * C * sizeof(float)) + align_up((size_t)B * C * sizeof(float));
 }
 
@@ -512,11 +527,16 @@ template <class T, class F> static int rec_shape(int C, const RecPlan& pl, F f) 
 template <class Q, class U> static bool rec_near(const Rows<U>& r, int C) {
     return r.row >= 0 && r.row < (1l << 31) / (Q::TILE * (long)sizeof(U)) && C < 1 << 28;
 }
+// Whether a result's rows are whole lines.  Past the caches those are 10 % faster (16 x 3999 x 512 fp32 forward 85 and 94 us), parts of
+// lines, which only meet in a cache, up to 45 % slower (16 x 3999 x 501 fp32 backward 212 and 147 us).
+template <class U> static bool rec_lines(const Rows<U>& r) {
+    return ((uintptr_t)r.p | (r.row | r.batch) * sizeof(U)) % 128 == 0;
+}
 
 template <class T>
 static int run_recurrence(Rows<const T> x, Rows<const T> gate, const float* h0, const int* lengths, Rows<T> h, float* last, float* saved,
                           int B, int S, int C, bool reverse, void* ws, hipStream_t st) {
-    RecPlan pl = rec_plan(B, S, C, sizeof(T));
+    RecPlan pl = rec_plan(B, S, C, sizeof(T), false);
     Arena arena(ws, ~(size_t)0);
     float* agg = pl.pieces > 1 ? arena.take<float>((size_t)B * pl.pieces * 2 * C) : nullptr;
     float* kept = pl.pieces > 1 ? arena.take<float>((size_t)B * C) : nullptr;
@@ -525,6 +545,7 @@ static int run_recurrence(Rows<const T> x, Rows<const T> gate, const float* h0, 
     return rec_shape<T>(C, pl, [&](auto q) {
         typedef decltype(q) Q;
         pl.near = rec_near<Q>(x, C) && rec_near<Q>(gate, C) && rec_near<Q>(h, C);
+        pl.past = rec_lines(h);
         if constexpr (Q::W == REC_WIDE)
             if (pl.pieces > 1) rec_piece_kernel<false, Q><<<grid, 64 * Q::W, 0, st>>>(x, gate, h0, lengths, agg, kept, pl, S, C, reverse);
         rec_forward_kernel<Q><<<grid, 64 * Q::W, 0, st>>>(x, gate, pl.pieces > 1 ? kept : h0, lengths, h, last, saved, agg, pl, S, C, reverse);
@@ -536,7 +557,7 @@ template <class T>
 static int run_recurrence_backward(Rows<const T> dh, Rows<const T> x, Rows<const T> gate, const float* saved, const float* dlast,
                                    const int* lengths, Rows<T> dx, Rows<T> dgate, float* dh0, int B, int S, int C, bool reverse, void* ws,
                                    hipStream_t st) {
-    RecPlan pl = rec_plan(B, S, C, sizeof(T));
+    RecPlan pl = rec_plan(B, S, C, sizeof(T), true);
     Arena arena(ws, ~(size_t)0);
     float* agg = pl.pieces > 1 ? arena.take<float>((size_t)B * pl.pieces * 2 * C) : nullptr;
     float* kept = pl.pieces > 1 ? arena.take<float>((size_t)B * C) : nullptr;
@@ -545,6 +566,7 @@ static int run_recurrence_backward(Rows<const T> dh, Rows<const T> x, Rows<const
     return rec_shape<T>(C, pl, [&](auto q) {
         typedef decltype(q) Q;
         pl.near = rec_near<Q>(dh, C) && rec_near<Q>(x, C) && rec_near<Q>(gate, C) && rec_near<Q>(dx, C) && rec_near<Q>(dgate, C);
+        pl.past = rec_lines(dx) && rec_lines(dgate);
         if constexpr (Q::W == REC_WIDE)
             if (pl.pieces > 1) rec_piece_kernel<true, Q><<<grid, 64 * Q::W, 0, st>>>(dh, gate, dlast, lengths, agg, kept, pl, S, C, reverse);
         rec_backward_kernel<Q><<<grid, 64 * Q::W, 0, st>>>(dh, x, gate, saved, pl.pieces > 1 ? kept : dlast, lengths, dx, dgate, dh0, agg,

@@ -321,7 +321,11 @@ def gated_recurrence(x, gate, h0=None, lengths=None, reverse=False, last=None, s
     h0p, lp = _aside(h0, "h0", (B, C), dev), _aside(lengths, "lengths", (B,), dev, torch.int32)
     if last is None:
         last = torch.empty((B, C), device=dev)
-    lastp = _aside(last, "last", (B, C), dev)
+        lastp = last.data_ptr()
+    else:
+        lastp = _aside(last, "last", (B, C), dev)
+        if any(u is not None and _clash(last, u) for u in (x, gate)) or (h0 is not None and _clash(last, h0) and lastp != h0p):
+            raise ValueError("last: the output shares memory with another operand")
     h = torch.empty((B, S, C), dtype=x.dtype, device=dev)
     saved = torch.empty((B, -(-S // _lib.RECURRENCE_SAVE), C), device=dev) if save else None
     if B and S:
@@ -330,7 +334,7 @@ def gated_recurrence(x, gate, h0=None, lengths=None, reverse=False, last=None, s
               (*xr, *gr, h0p, lp, h.data_ptr(), S * C, C, lastp, saved.data_ptr() if save else None, B, S, C, int(reverse), t))
     elif h0 is None:
         last.zero_()
-    elif last is not h0:
+    elif lastp != h0p:
         last.copy_(h0)
     return h, last, saved
 
