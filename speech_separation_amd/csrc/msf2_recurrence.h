@@ -20,7 +20,7 @@ constexpr int REC_WIDE = 8;                  // waves of a workgroup, where a se
 
 // How the work is dealt out: `slices` of channels by `pieces` of `piece` frames by utterances.
 struct RecPlan {
-    int lanes, slices, pieces, waves, piece;
+    int vec, lanes, slices, pieces, waves, piece;
     bool near;                               // a tile's rows span less than 2^32 bytes in every operand
     bool past;                               // results go past the caches
 };
@@ -271,7 +271,7 @@ template <bool BACK, class Q>
 __global__ __launch_bounds__(64 * Q::W) void rec_piece_kernel(Rows<const typename Q::T> u, Rows<const typename Q::T> gate, const float* start,
                                                               const int* lengths, float* agg, float* kept, RecPlan pl, int S, int C, bool reverse) {
     typedef typename Q::T T;
-    constexpr int V = Q::V, R = 8;
+    constexpr int V = Q::V, R = Q::R;
     __shared__ Run<V> runs[Q::W][Q::LC];
     const RecPlace<Q> at(pl, lengths, S, C);
     if (at.p == (BACK ? pl.pieces - 1 : 0) && at.first()) {
@@ -483,9 +483,14 @@ __global__ __launch_bounds__(64 * Q::W) void rec_backward_kernel(Rows<const type
     if (dh0 && t0 == 0 && at.first()) rec_store<V>(dh0 + (long)at.b * C + at.c, at.own, carry);
 }
 
-constexpr int REC_V = 2, REC_R = 8;                            // channels and frames a thread
+// A thread takes 16 values: `vec` channels by 16 / vec frames, 8 bytes of a frame, except that the backward pass of the 16-bit types
+// takes 4 of an even width (64 x 3999 x 512 bf16 backward, 4 and 8 bytes: 260 and 279 us; x 501, where every other row is off the
+// 4-byte grid: 430 and 371; forward 163 and 159, 236 and 212).  By width and not by the operands' alignment, so that a slice of a wider
+// tensor gives the same bits as its copy.
+constexpr int REC_VALUES = 16;
+static inline bool rec_pairs(int bytes, int C, bool backward) { return bytes == 2 && backward && C % 2 == 0; }
 // the short form's waves: as many as reach from one saved state to the next
-constexpr int rec_short(int lanes) { return std::max(1, REC_SAVE / (64 / lanes * REC_R)); }
+constexpr int rec_short(int lanes, int rows) { return std::max(1, REC_SAVE / (64 / lanes * rows)); }
 
 // Slices of 256 bytes of a frame where that leaves a workgroup for every CU, else of 128: two lines a row reach 4.9 TB/s, one 4.3
 // (64 x 3999 x 512 bf16 forward: 162 and 184 us).  A sequence is cut into pieces, each read twice, where whole sequences occupy
@@ -494,11 +499,12 @@ constexpr int rec_short(int lanes) { return std::max(1, REC_SAVE / (64 / lanes *
 // workgroups, 88 in 512; forward 64 and 58).  Two tiles in a row take less time than another launch does (8.3 and 9.5 us at 4 x 512 x 256
 // fp32), three take more (10.8 and 9.6).
 static inline RecPlan rec_plan(int B, int S, int C, int bytes, bool backward) {
-    const int V = C >= REC_V ? REC_V : 1;
+    const int vec = rec_pairs(bytes, C, backward) ? 2 : 8 / bytes, V = C >= vec ? vec : 1, rows = REC_VALUES / vec;
     RecPlan pl;
-    pl.lanes = 128 / bytes;
+    pl.vec = V;
+    pl.lanes = 256 / (vec * bytes);
     if (V == 1 || (long)B * ((C + pl.lanes * V - 1) / (pl.lanes * V)) < 256) pl.lanes /= 2;
-    const int wave = 64 / pl.lanes * REC_R, few = rec_short(pl.lanes);
+    const int wave = 64 / pl.lanes * rows, few = rec_short(pl.lanes, rows);
     pl.slices = (C + pl.lanes * V - 1) / (pl.lanes * V);
     pl.waves = S <= few * wave ? few : REC_WIDE;
     const long tile = (long)pl.waves * wave, tiles = (S + tile - 1) / tile, seqs = (long)B * pl.slices;
@@ -515,13 +521,18 @@ static inline size_t rec_ws_bytes(int B, int S, int C, int bytes, bool backward)
 }
 
 // f(RecShape) of the form that the plan names
-template <class T, int V, int LC, class F> static int rec_waves(const RecPlan& pl, F f) {
-    return pl.waves == REC_WIDE ? f(RecShape<T, V, LC, REC_R, REC_WIDE>()) : f(RecShape<T, V, LC, REC_R, rec_short(LC)>());
+template <class T, int V, int LC, int R, class F> static int rec_waves(const RecPlan& pl, F f) {
+    return pl.waves == REC_WIDE ? f(RecShape<T, V, LC, R, REC_WIDE>()) : f(RecShape<T, V, LC, R, rec_short(LC, R)>());
 }
-template <class T, class F> static int rec_shape(int C, const RecPlan& pl, F f) {
-    constexpr int LC = 128 / sizeof(T);
-    if (C < REC_V) return rec_waves<T, 1, LC / 2>(pl, f);
-    return pl.lanes == LC ? rec_waves<T, REC_V, LC>(pl, f) : rec_waves<T, REC_V, LC / 2>(pl, f);
+template <class T, int VEC, class F> static int rec_lanes(const RecPlan& pl, F f) {
+    constexpr int LC = 256 / (VEC * sizeof(T)), R = REC_VALUES / VEC;
+    if (pl.vec == 1) return rec_waves<T, 1, LC / 2, R>(pl, f);
+    return pl.lanes == LC ? rec_waves<T, VEC, LC, R>(pl, f) : rec_waves<T, VEC, LC / 2, R>(pl, f);
+}
+template <class T, bool BACK, class F> static int rec_shape(const RecPlan& pl, int C, F f) {
+    if constexpr (BACK && sizeof(T) == 2)
+        if (rec_pairs(sizeof(T), C, true)) return rec_lanes<T, 2>(pl, f);
+    return rec_lanes<T, 8 / sizeof(T)>(pl, f);
 }
 // whether a tile of an operand can be addressed by 32-bit offsets
 template <class Q, class U> static bool rec_near(const Rows<U>& r, int C) {
@@ -542,7 +553,7 @@ static int run_recurrence(Rows<const T> x, Rows<const T> gate, const float* h0, 
     float* kept = pl.pieces > 1 ? arena.take<float>((size_t)B * C) : nullptr;
     const long grid = (long)B * pl.pieces * pl.slices;
     if (grid > 0x7fffffff) return MSF2_ERR_ARG;
-    return rec_shape<T>(C, pl, [&](auto q) {
+    return rec_shape<T, false>(pl, C, [&](auto q) {
         typedef decltype(q) Q;
         pl.near = rec_near<Q>(x, C) && rec_near<Q>(gate, C) && rec_near<Q>(h, C);
         pl.past = rec_lines(h);
@@ -563,7 +574,7 @@ static int run_recurrence_backward(Rows<const T> dh, Rows<const T> x, Rows<const
     float* kept = pl.pieces > 1 ? arena.take<float>((size_t)B * C) : nullptr;
     const long grid = (long)B * pl.pieces * pl.slices;
     if (grid > 0x7fffffff) return MSF2_ERR_ARG;
-    return rec_shape<T>(C, pl, [&](auto q) {
+    return rec_shape<T, true>(pl, C, [&](auto q) {
         typedef decltype(q) Q;
         pl.near = rec_near<Q>(dh, C) && rec_near<Q>(x, C) && rec_near<Q>(gate, C) && rec_near<Q>(dx, C) && rec_near<Q>(dgate, C);
         pl.past = rec_lines(dx) && rec_lines(dgate);
