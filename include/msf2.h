@@ -347,7 +347,7 @@ int msf2_pit_si_snr_noalloc(const float* est, const float* src, float* si_snr, f
 #define MSF2_ACT_SIGMOID 2
 #define MSF2_ACT_RELU 3
 
-/* y = act(norm(x)), or norm(act(x)) with act_first != 0 (the order of TCNBlock.net, mossformer2_block.py:513-519);
+/* y = act(norm(x)), or norm(act(x)) with act_first != 0 (the order of TCNBlock.net, mossformer2_block.py:508-531);
  * norm: per utterance and group of C / groups neighbouring channels, over the utterance's frames and the group's
  * channels, biased variance + eps, then gamma[c], beta[c] (null: 1, 0).
  *   stats [B][groups][2] = (mean, 1 / sqrt(var + eps)) of act_first ? act(x) : x; (0, 0) for an empty utterance.

@@ -257,7 +257,7 @@ def _call(name, dev, ws_bytes, args):
 def group_norm_act(x, gamma, beta, groups, eps=1e-5, act=_lib.ACT_NONE, act_first=False, lengths=None):
     """y = act(norm(x)) of x [B, S, C], or norm(act(x)) with act_first: (y, stats [B, groups, 2] = mean and 1/sqrt(var + eps)
     for the backward pass).  act: _lib.ACT_*.  gamma, beta: fp32 [C] or None; lengths: int32 [B] or None, the frames of each
-    utterance: frames past them count for nothing and are zero in y.  Reference: TCNBlock.net, mossformer2_block.py:513-519."""
+    utterance: frames past them count for nothing and are zero in y.  Reference: TCNBlock.net, mossformer2_block.py:508-531."""
     lib = _lib.load()
     xr = _rows(x, "x")
     B, S, C = x.shape
