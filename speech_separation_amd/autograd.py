@@ -36,7 +36,7 @@ class _GroupNormAct(torch.autograd.Function):
 class _GatedRecurrence(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, h0, lengths, reverse):
-        h, last, saved = ops.gated_recurrence(x, gate, h0, lengths, reverse, save=True)
+        h, last, saved = ops.gated_recurrence(x, gate, h0, lengths, reverse, save=any(ctx.needs_input_grad))
         ctx.save_for_backward(x, gate, saved, lengths)
         ctx.reverse = reverse
         return h, last

@@ -232,6 +232,14 @@ def _out_rows(t, name, like, same_type=True, apart=(), same=()):
     return r
 
 
+def _written(*ts):
+    """Tensors of the caller's that a kernel is about to write: autograd is told, as by any operation in place."""
+    for t in ts:
+        if t.requires_grad and (t.is_leaf or torch.is_grad_enabled()):
+            raise ValueError("a tensor that requires a gradient cannot be written in place here")
+        torch.autograd.graph.increment_version(t)
+
+
 def _aside(t, name, shape, device, dtype=torch.float32):
     """Address of a contiguous side operand (None: null)."""
     if t is None:
@@ -326,6 +334,7 @@ def gated_recurrence(x, gate, h0=None, lengths=None, reverse=False, last=None, s
         lastp = _aside(last, "last", (B, C), dev)
         if any(u is not None and _clash(last, u) for u in (x, gate)) or (h0 is not None and _clash(last, h0) and lastp != h0p):
             raise ValueError("last: the output shares memory with another operand")
+        _written(last)
     h = torch.empty((B, S, C), dtype=x.dtype, device=dev)
     saved = torch.empty((B, -(-S // _lib.RECURRENCE_SAVE), C), device=dev) if save else None
     if B and S:
@@ -356,6 +365,7 @@ def gated_recurrence_backward(dh, x, gate, saved, dlast=None, lengths=None, reve
         dx, dgate = out
         dxr = _out_rows(dx, "dx", x, apart=(dh, x, gate, saved, dlast, dgate))
         dgr = _out_rows(dgate, "dgate", x, apart=(dh, x, gate, saved, dlast))
+        _written(dx, dgate)
     dlp, lp = _aside(dlast, "dlast", (B, C), dev), _aside(lengths, "lengths", (B,), dev, torch.int32)
     savedp = _aside(saved, "saved", (B, -(-S // _lib.RECURRENCE_SAVE), C), dev)
     if savedp is None:
@@ -400,7 +410,9 @@ def dropout(x, p, rng, site=0, residual=None, out=None):
         raise ValueError("x, residual: expected tensors")
     if out is not None:
         _rows(x, "x")
-        return _dropout(x, p, rng, site, residual, out, _out_rows(out, "out", x, same_type=False, apart=(rng,), same=(x, residual)))
+        yr = _out_rows(out, "out", x, same_type=False, apart=(rng,), same=(x, residual))
+        _written(out)
+        return _dropout(x, p, rng, site, residual, out, yr)
     return _dropout(x, p, rng, site, residual, torch.empty(x.shape, dtype=(x if residual is None else residual).dtype, device=x.device))
 
 

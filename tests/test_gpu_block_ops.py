@@ -67,6 +67,11 @@ NORM = [  # B, S, C, groups, type, act, act_first, lengths, strides
     (1, 9000, 8, 1, F32, 1, False, None, "plain"),
     (300, 3, 64, 4, F32, 1, False, None, "plain"),
     (2, 3000, 1024, 8, BF16, 1, False, None, "plain"),
+    (2, 20, 4100, 1, F32, 1, False, "ends", "plain"),
+    (2, 20, 4100, 4100, BF16, 2, False, None, "plain"),     # every channel a group, more of them than a workgroup takes
+    (1, 70, 9001, 1, FP16, 0, False, None, "wide"),
+    (3, 200, 2, 1, BF16, 1, True, "ends", "plain"),         # frames narrower than a vector
+    (3, 200, 1, 1, F32, 2, False, None, "wide"),
 ]
 
 
@@ -167,6 +172,11 @@ REC = [  # B, S, C, type, lengths, reverse, strides, h0, dlast
     (33, 257, 96, BF16, "ends", False, "plain", False, True),
     (1, 3000, 513, BF16, None, False, "plain", True, True),
     (8, 513, 512, FP16, "rolled", True, "wide", True, True),
+    (2, 70, 4100, BF16, "ends", False, "plain", True, True),
+    (2, 300, 3, BF16, None, True, "wide", True, True),
+    (300, 40, 129, F32, "ends", False, "frames", True, True),
+    (70000, 2, 5, FP16, "ends", True, "plain", True, True),
+    (40, 300, 501, BF16, "ends", False, "plain", False, True),
 ]
 
 
@@ -252,6 +262,18 @@ def test_gated_recurrence_state_in_place_over_a_long_sequence():
         assert torch.equal(h, h2) and torch.equal(last, state) and torch.equal(saved, saved2)
 
 
+@pytest.mark.parametrize("C,dtype", [(33, F32), (65, BF16), (129, F32), (131, FP16)])
+def test_gated_recurrence_state_in_place_where_slices_share_channels(C, dtype):
+    """Widths whose last lanes are moved left over channels of the slice before, which another workgroup may have finished."""
+    g = torch.Generator().manual_seed(15)
+    x, gate, dh, h0, dlast = to_dev(*rec_inputs(g, 70, 90, C, dtype, None))
+    h, last, saved = ops.gated_recurrence(x, gate, h0, save=True)
+    for _ in range(5):
+        state = h0.clone()
+        h2, _, saved2 = ops.gated_recurrence(x, gate, state, last=state, save=True)
+        assert torch.equal(h, h2) and torch.equal(last, state) and torch.equal(saved, saved2)
+
+
 def test_gated_recurrence_gradients_into_one_tensor():
     g = torch.Generator().manual_seed(14)
     both = randn(g, 3, 200, 2 * 40, dtype=BF16).to(DEV)
@@ -317,6 +339,15 @@ def test_dropout_in_place():
     assert torch.equal(wide[..., :44], x) and not bool(wide[..., 44:50].any()) and not bool(wide[..., 94:].any())
 
 
+def test_dropout_many_utterances_that_do_not_follow_one_another():
+    """More utterances than a grid's second dimension counts."""
+    B, S, C = 70000, 2, 9
+    x = place(torch.arange(B * S * C, dtype=F32).view(B, S, C) % 97 - 48, "frames")
+    rng = torch.tensor([8, 9], device=DEV)
+    y = ops.dropout(x, 0.4, rng, 1)
+    close(y, *oracle.dropout(x.cpu(), 0.4, 8, 9, 1))
+
+
 # ------------------------------------------------------------------ all of them
 def test_refusals():
     x, f64, i32 = torch.zeros(2, 3, 8, device=DEV), torch.zeros(2, 3, 8, dtype=torch.float64, device=DEV), torch.zeros(2, dtype=torch.int32, device=DEV)
@@ -342,9 +373,39 @@ def test_refusals():
         lambda: ops.dropout(half, 0.1, rng, residual=x.to(FP16)), lambda: ops.dropout(x, 0.1, rng, residual=x[:, :2]), lambda: ops.dropout(x, 0.1, rng, residual=3.0),
         lambda: ops.dropout(x[:, :2], 0.1, rng, out=x[:, 1:]), lambda: ops.dropout_backward(half, 0.1, rng, dtype=FP16), lambda: ops.dropout_backward(None, 0.1, rng),
     ]
+    leaf = torch.zeros(2, 8, device=DEV, requires_grad=True)
+    dx = torch.empty_like(x)
+    bad += [lambda: ops.gated_recurrence(x, x, last=leaf), lambda: ops.gated_recurrence(x, x, hs, last=x.view(-1)[8:24].view(2, 8)),
+            lambda: ops.gated_recurrence_backward(x, x, x, sv, out=(dx, dx)), lambda: ops.dropout(x, 0.1, rng, out=x.clone().requires_grad_()),
+            lambda: ops.dropout(x, 0.1, rng, out=torch.empty(2, 3, 4, device=DEV)), lambda: ops.gated_recurrence_backward(x, x, x, sv, out=(dx, half))]
     for f in bad:
         with pytest.raises(ValueError):
             f()
+
+
+def test_writing_in_place_is_noticed_by_autograd():
+    w = torch.randn(2, 3, 8, device=DEV, requires_grad=True)
+    r = torch.randn(2, 3, 8, device=DEV)
+    y = (w * r).sum()
+    ops.dropout(torch.randn(2, 3, 8, device=DEV), 0.1, torch.tensor([1, 2], device=DEV), residual=r, out=r)
+    with pytest.raises(RuntimeError):
+        y.backward()
+
+
+def test_autograd_refuses_its_backward_under_capture(monkeypatch):
+    x = torch.randn(2, 3, 8, device=DEV, requires_grad=True)
+    outs = [autograd.group_norm_act(x, None, None, 2), autograd.gated_recurrence(x, x)[0], autograd.dropout(x, 0.1, torch.tensor([1, 2], device=DEV))]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    for y in outs:
+        with pytest.raises(RuntimeError):
+            y.sum().backward()
+
+
+def test_autograd_without_gradients_saves_nothing():
+    x = torch.randn(2, 40, 8, device=DEV)
+    with torch.no_grad():
+        h, last = autograd.gated_recurrence(x, x)
+    assert torch.equal(h, ops.gated_recurrence(x, x)[0]) and not h.requires_grad
 
 
 def block(x, w, lengths, state, rng):
@@ -547,6 +608,22 @@ def test_rows_beyond_32_bits():
     want = oracle.recurrence(x[:, -90:].cpu(), gate[:, -90:].cpu(), torch.ones(1, C))        # 0.5^60 of what came before is left
     close(h[:, -30:], want["h"][0][:, -30:], want["h"][1][:, -30:] + 1e-12)
     close(last, want["last"][0], want["last"][1] + 1e-12)
+
+
+def test_group_norm_act_beyond_32_bits():
+    S, C = 33000000, 66
+    x = torch.empty(1, S, C, dtype=BF16, device=DEV)
+    x.fill_(1.0)
+    x[..., 1::2] = -1.0
+    y, stats = ops.group_norm_act(x, None, None, 1)
+    r = 1 / (1 + 1e-5) ** 0.5
+    assert abs(float(stats[0, 0, 0])) < 1e-6 and abs(float(stats[0, 0, 1]) - r) < 1e-6
+    assert bool((y[0, -50:].float().abs() == torch.tensor(r).to(BF16).float().item()).all()) and bool((y[0, -50:, 0] > 0).all())
+    dy = torch.zeros_like(x)
+    dy[0, -1, 0] = 1.0
+    dx, dgamma, dbeta = ops.group_norm_act_backward(dy, x, torch.ones(C, device=DEV), torch.zeros(C, device=DEV), stats, 1)
+    assert abs(float(dx[0, -1, 0]) - 1) < 0.01 and abs(float(dx[0, -1, 1])) < 1e-6       # one of 2 10^9 values
+    assert abs(float(dgamma[0]) - r) < 1e-5 and float(dbeta[0]) == 1.0 and not bool(dbeta[1:].any())
 
 
 def _tail_keep(S, C, rows):
