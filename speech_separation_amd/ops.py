@@ -237,7 +237,8 @@ def _written(*ts):
     for t in ts:
         if t.requires_grad and (t.is_leaf or torch.is_grad_enabled()):
             raise ValueError("a tensor that requires a gradient cannot be written in place here")
-        torch.autograd.graph.increment_version(t)
+        if not t.is_inference():             # those have no version to count
+            torch.autograd.graph.increment_version(t)
 
 
 def _aside(t, name, shape, device, dtype=torch.float32):

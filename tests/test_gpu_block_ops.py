@@ -401,6 +401,16 @@ def test_autograd_refuses_its_backward_under_capture(monkeypatch):
             y.sum().backward()
 
 
+def test_inference_mode():
+    with torch.inference_mode():
+        x, state, rng = torch.randn(2, 3, 8, device=DEV), torch.zeros(2, 8, device=DEV), torch.tensor([1, 2], device=DEV)
+        h, last, _ = ops.gated_recurrence(x, x, state.clone())
+        assert torch.equal(ops.gated_recurrence(x, x, state, last=state)[0], h) and torch.equal(state, last)
+        y = ops.dropout(h, 0.1, rng, residual=x)
+        assert torch.equal(ops.dropout(h, 0.1, rng, residual=x, out=x), y)
+        assert torch.equal(autograd.gated_recurrence(x, x)[0], ops.gated_recurrence(x, x)[0])
+
+
 def test_autograd_without_gradients_saves_nothing():
     x = torch.randn(2, 40, 8, device=DEV)
     with torch.no_grad():
