@@ -329,54 +329,66 @@ __device__ __forceinline__ float4 bf16x4_ld(const unsigned short* p) {
                        __builtin_bit_cast(float, h.y << 16), __builtin_bit_cast(float, h.y & 0xffff0000u));
 }
 constexpr int DW16_TS = 32;      // frames per block of the bf16 kernel: 48 row reads per 32 results
-// Input rows R0 .. R1 - 1 of a tile into every result row they reach.  Two halves of the tile's rows, because the
-// compiler gives up unrolling one loop over all 48 (64 multiply-adds a row), and what it leaves rolled indexes acc in memory.
-template <int R0, int R1>
-__device__ __forceinline__ void dw16_rows(const unsigned short* __restrict__ xb, int ldx, int s0, int S, const float4 (&w)[17],
-                                          float4 (&acc)[DW16_TS]) {
+// The tile's 48 input rows in six parts of 8, from row s0 - 8 on: the loads of part P + 3 go out, part P is added into every result
+// row that it reaches, and the result rows that are complete by then are stored, so that at most 24 of them are held.  (One loop over
+// all rows is more than the compiler unrolls: what it leaves rolled indexes the results in memory.)
+template <int P> struct Dw16Part {
+    static __device__ __forceinline__ void load(uint2 (&raw)[6][8], const unsigned short* xb, int ldx, int s0, int S) {
 #pragma unroll
-    for (int r = R0; r < R1; ++r) {
-        const int s = s0 + r;
-        const float inb = (s >= 0 && s < S) ? 1.f : 0.f;      // see dwconv17_kernel
-        float4 xv = bf16x4_ld(xb + (long)min(max(s, 0), S - 1) * ldx);
-        xv.x *= inb; xv.y *= inb; xv.z *= inb; xv.w *= inb;
+        for (int j = 0; j < 8; ++j)
+            raw[P][j] = *reinterpret_cast<const uint2*>(xb + (long)min(max(s0 - 8 + 8 * P + j, 0), S - 1) * ldx);
+    }
+    static __device__ __forceinline__ void run(uint2 (&raw)[6][8], const unsigned short* xb, int ldx, int s0, int S, const float4 (&w)[17],
+                                               float4 (&acc)[DW16_TS], unsigned short* yb, int ldy) {
+        if constexpr (P + 3 < 6) Dw16Part<P + 3>::load(raw, xb, ldx, s0, S);
 #pragma unroll
-        for (int k = 0; k < 17; ++k) {
-            const int o = r - k + 8;             // the result row this input row feeds through tap k
-            if (o >= 0 && o < DW16_TS) {
-                acc[o].x += w[k].x * xv.x; acc[o].y += w[k].y * xv.y;
-                acc[o].z += w[k].z * xv.z; acc[o].w += w[k].w * xv.w;
+        for (int j = 0; j < 8; ++j) {
+            const int r = 8 * P + j - 8, s = s0 + r;
+            const bool in = s >= 0 && s < S;             // the same for the whole block
+            const unsigned hx = in ? raw[P][j].x : 0u, hy = in ? raw[P][j].y : 0u;
+            const float4 xv = make_float4(__builtin_bit_cast(float, hx << 16), __builtin_bit_cast(float, hx & 0xffff0000u),
+                                          __builtin_bit_cast(float, hy << 16), __builtin_bit_cast(float, hy & 0xffff0000u));
+#pragma unroll
+            for (int k = 0; k < 17; ++k) {
+                const int o = r - k + 8;                 // the result row this input row feeds through tap k
+                if (o >= 0 && o < DW16_TS) {
+                    if (k == 0) acc[o] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    acc[o].x += w[k].x * xv.x; acc[o].y += w[k].y * xv.y;
+                    acc[o].z += w[k].z * xv.z; acc[o].w += w[k].w * xv.w;
+                }
             }
         }
+        if constexpr (P >= 2) {
+#pragma unroll
+            for (int o = 8 * (P - 2); o < 8 * (P - 1); ++o)
+                if (s0 + o < S) {
+                    uint2 h;
+                    h.x = pk_bf16_pair(acc[o].x, acc[o].y);
+                    h.y = pk_bf16_pair(acc[o].z, acc[o].w);
+                    *reinterpret_cast<uint2*>(yb + (long)(s0 + o) * ldy) = h;
+                }
+        }
+        if constexpr (P + 1 < 6) Dw16Part<P + 1>::run(raw, xb, ldx, s0, S, w, acc, yb, ldy);
     }
-}
+};
+static_assert(DW16_TS == 32, "six parts of 8 rows: the tile and 8 rows on either side");
 __global__ __launch_bounds__(128, 2) void dwconv17_bf16_kernel(const unsigned short* __restrict__ x, int ldx,
                                                             const float* __restrict__ dw, unsigned short* __restrict__ y,
                                                             int ldy, int S, int C) {
     const int cq = blockIdx.x * 128 + threadIdx.x;
     if (cq >= (C >> 2)) return;
     const int b = blockIdx.z, s0 = blockIdx.y * DW16_TS;
+    const unsigned short* xb = x + (long)b * S * ldx + 4 * cq;
+    uint2 raw[6][8];
+    Dw16Part<0>::load(raw, xb, ldx, s0, S);
+    Dw16Part<1>::load(raw, xb, ldx, s0, S);
+    Dw16Part<2>::load(raw, xb, ldx, s0, S);
     float4 w[17];
 #pragma unroll
     for (int k = 0; k < 17; ++k) w[k] = *reinterpret_cast<const float4*>(dw + k * C + 4 * cq);
     w[8].x += 1.f; w[8].y += 1.f; w[8].z += 1.f; w[8].w += 1.f;      // y = x + conv(x): the centre tap carries the identity
     float4 acc[DW16_TS];
-#pragma unroll
-    for (int o = 0; o < DW16_TS; ++o) acc[o] = make_float4(0.f, 0.f, 0.f, 0.f);
-    const unsigned short* xb = x + (long)b * S * ldx + 4 * cq;
-    dw16_rows<-8, DW16_TS / 2>(xb, ldx, s0, S, w, acc);
-    dw16_rows<DW16_TS / 2, DW16_TS + 8>(xb, ldx, s0, S, w, acc);
-    unsigned short* yb = y + (long)b * S * ldy + 4 * cq;
-#pragma unroll
-    for (int o = 0; o < DW16_TS; ++o) {
-        const int s = s0 + o;
-        if (s < S) {
-            uint2 h;
-            h.x = pk_bf16_pair(acc[o].x, acc[o].y);
-            h.y = pk_bf16_pair(acc[o].z, acc[o].w);
-            *reinterpret_cast<uint2*>(yb + (long)s * ldy) = h;
-        }
-    }
+    Dw16Part<0>::run(raw, xb, ldx, s0, S, w, acc, y + (long)b * S * ldy + 4 * cq, ldy);
 }
 
 // ---- OffsetScale + rotary -> quad_q/256, lin_q, quad_k, lin_k ----------------
@@ -965,6 +977,9 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2, 4))) void
     // tap by tap (the taps of a thread's channels are the same for every frame: cache-resident loads)
 #pragma unroll
     for (int k = 0; k < FS_K; ++k) {
+        // NIN = 2: taps are loaded 4 ahead at most.  All 39 pairs at once, beside the window, are more than 256 registers hold
+        // (49 spilled and twice the time).
+        if (NIN == 2 && k % 4 == 0) asm volatile("" ::: "memory");
         float2 wv;              // NIN = 1: w[k][c .. c+1]; NIN = 2: (w[k][0][c], w[k][1][c])
         if (NIN == 1) wv = *reinterpret_cast<const float2*>(w + (long)k * C + c);
         else wv = make_float2(w[((long)k * 2 + 0) * C + c], w[((long)k * 2 + 1) * C + c]);
