@@ -2,8 +2,9 @@
 //
 // Memory-bound: x (and dy) once for the sums and once for the result, which is three passes over an activation forward and five
 // backward.  64 x 3999 x 512 bf16 forward 136 us (5.8 TB/s of what it moves; a copy of 1 GiB reaches 5.1 here), 16 x 3999 x 512 fp32
-// forward 75 us and backward 110 us (5.3 and 6.0 TB/s); small calls are two launches of 5 us.  A workgroup takes `width` neighbouring channels of some
-// frames of one utterance; lanes run over channels first, so a frame's part of a slice is whole lines.  Its sums go to the
+// forward 75 us and backward 110 us (5.3 and 6.0 TB/s); small calls are two launches of 5 us.
+//
+// A workgroup takes `width` neighbouring channels, the whole frame where it can, of some frames of one utterance.  Its sums go to the
 // workspace per (chunk of frames, slice, group), a group's sums lie in every slice that it touches, and the workgroups that use a
 // group's sums join them themselves: no atomics, the same order every time.
 //
@@ -25,7 +26,8 @@ constexpr int GN_T = 512;                    // most threads of a workgroup
 constexpr int GN_LANES = 128;                // most lanes over the channels of a frame
 constexpr int GN_ROWS = 64;                  // frames a thread sums in 32 bits at most
 
-// Division of the work: `slices` of `width` channels (`lanes` x V) by `chunks` of `rows` frames by utterances.  Within a slice a group counts from the first that touches it; at most `local` groups do.
+// Division of the work: `slices` of `width` channels (`lanes` x V) by `chunks` of `rows` frames by utterances.  Within a slice a
+// group counts from the first that touches it; at most `local` groups do.
 struct GnPlan {
     int lanes, step, threads, width, slices, chunks, rows, local, D;     // step: frames that a workgroup takes side by side
     Divider by_D, by_width;
@@ -35,9 +37,11 @@ struct GnPlan {
 };
 
 // A thread's place.  The lane of the last channels is moved left to end with the row, so that every access is a whole vector: what
-// it shares with its neighbour (below `own`) counts for nothing in sums and is stored twice with the same value.
+// it shares with its neighbour (below `own`) counts for nothing in sums and is stored twice with the same value -- but for the lane that
+// is moved into the slice before (`astray`), whose groups this workgroup does not know: it stores its own channels only.
 template <int V> struct GnPlace {
     int b, slice, chunk, c, r0, step, have, own;
+    bool astray;
     __device__ GnPlace(const GnPlan& pl, unsigned block, int C) {
         slice = block % pl.slices;
         const unsigned rest = block / pl.slices;
@@ -49,6 +53,7 @@ template <int V> struct GnPlace {
         have = r0 < step ? min(C - c, V) : 0;        // channels of this lane, none or less past the row's end
         own = C >= V && have > 0 ? V - have : 0;
         c -= own;
+        astray = own && c < slice * pl.width;
     }
 };
 
@@ -67,16 +72,18 @@ template <int V> __device__ __forceinline__ void gn_channels(const float* p, int
         for (int v = 0; v < V; ++v) f[v] = p && c + v < C ? p[c + v] : none;
     }
 }
-template <int V> __device__ __forceinline__ void gn_of_groups(const float* pairs, const GnPlan& pl, int c, int C, float (&a)[V], float (&b)[V]) {
-    const int g = pl.group(min(c, C - 1));
-    if (pl.D % V == 0) {                     // one group holds them all
+// g0: the first group that `pairs` holds.
+template <int V>
+__device__ __forceinline__ void gn_of_groups(const float* pairs, int g0, const GnPlan& pl, int c, int C, float (&a)[V], float (&b)[V]) {
+    if (pl.D % V == 0) {                     // one group holds them all, and no lane is moved
+        const int g = pl.group(min(c, C - 1)) - g0;
         const float p = pairs[2 * g], q = pairs[2 * g + 1];
 #pragma unroll
         for (int v = 0; v < V; ++v) a[v] = p, b[v] = q;
     } else {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const int k = pl.group(min(c + v, C - 1));
+            const int k = max(pl.group(min(c + v, C - 1)) - g0, 0);
             a[v] = pairs[2 * k], b[v] = pairs[2 * k + 1];
         }
     }
@@ -86,9 +93,16 @@ template <int V> __device__ __forceinline__ void gn_of_groups(const float* pairs
 template <int V, class T> __device__ __forceinline__ typename VecOf<T, V>::type gn_load(const T* p, int C) {
     return C >= V ? load_vec<V>(p) : load_some<V>(p, C);
 }
-template <int V, class T> __device__ __forceinline__ void gn_store(T* p, int C, const float (&f)[V]) {
-    if (C >= V) store_vec<V, true>(p, f);
-    else store_some<V>(p, C, f);
+template <int V, class T> __device__ __forceinline__ void gn_store(T* p, int C, const GnPlace<V>& at, const float (&f)[V]) {
+    if (C < V) {
+        store_some<V>(p, C, f);
+    } else if (!at.astray) {
+        store_vec<V, true>(p, f);
+    } else {
+#pragma unroll
+        for (int v = 1; v < V; ++v)
+            if (v >= at.own) p[v] = (T)f[v];
+    }
 }
 // this thread's own channels into its row of a table [step][width]
 template <int V> __device__ __forceinline__ void gn_note(float* table, const GnPlan& pl, const GnPlace<V>& at, const float (&f)[V]) {
@@ -250,7 +264,7 @@ __global__ __launch_bounds__(GN_T) void gn_apply_kernel(Rows<const T> x, const f
         for (int i = threadIdx.x; i < 2 * groups; i += blockDim.x) stats[2 * ((long)at.b * G + g0) + i] = st[i];
     if (at.have <= 0) return;
     float mean[V], ga[V], be[V], rstd[V];
-    gn_of_groups<V>(st - 2 * g0, pl, at.c, C, mean, rstd);
+    gn_of_groups<V>(st, g0, pl, at.c, C, mean, rstd);
     gn_channels<V>(gamma, at.c, C, 1.f, ga);
     gn_channels<V>(beta, at.c, C, 0.f, be);
 #pragma unroll
@@ -270,7 +284,7 @@ __global__ __launch_bounds__(GN_T) void gn_apply_kernel(Rows<const T> x, const f
                 f[v] = act_f<POST, fine<T>()>(fmaf(act_f<PRE, fine<T>()>((float)w[j][v]) - mean[v], ga[v], be[v]));
                 if (s >= n) f[v] = 0.f;
             }
-            gn_store<V>(y.at(at.b, s) + at.c, C, f);
+            gn_store<V>(y.at(at.b, s) + at.c, C, at, f);
         }
     }
 }
@@ -298,7 +312,7 @@ __global__ __launch_bounds__(GN_T) void gn_grad_sums_kernel(Rows<const T> dy, Ro
     const bool some = at.have > 0 && s0 + at.r0 < s1;
     if (some) fetch(s0 + at.r0);
     float mean[V], rstd[V], ga[V], be[V], a1[V], a2[V];
-    gn_of_groups<V>(stats + 2 * (long)at.b * G, pl, at.c, C, mean, rstd);
+    gn_of_groups<V>(stats + 2 * (long)at.b * G, 0, pl, at.c, C, mean, rstd);
     gn_channels<V>(gamma, at.c, C, 1.f, ga);
     gn_channels<V>(beta, at.c, C, 0.f, be);
 #pragma unroll
@@ -412,8 +426,8 @@ __global__ __launch_bounds__(GN_T) void gn_dx_kernel(Rows<const T> dy, Rows<cons
     __syncthreads();
     if (at.have <= 0) return;
     float mean[V], rstd[V], ga[V], be[V], c1[V], c2[V];
-    gn_of_groups<V>(stats + 2 * (long)at.b * G, pl, at.c, C, mean, rstd);
-    gn_of_groups<V>(st - 2 * g0, pl, at.c, C, c1, c2);
+    gn_of_groups<V>(stats + 2 * (long)at.b * G, 0, pl, at.c, C, mean, rstd);
+    gn_of_groups<V>(st, g0, pl, at.c, C, c1, c2);
     gn_channels<V>(gamma, at.c, C, 1.f, ga);
     gn_channels<V>(beta, at.c, C, 0.f, be);
     for (int r = s0 + at.r0; r < s1; r += U * at.step) {
@@ -433,7 +447,7 @@ __global__ __launch_bounds__(GN_T) void gn_dx_kernel(Rows<const T> dy, Rows<cons
                 f[v] = rstd[v] * (fmaf(dz, ga[v], -c1[v]) - xh * c2[v]) * act_grad_f<PRE, fine<T>()>(xv);
                 if (s >= n) f[v] = 0.f;
             }
-            gn_store<V>(dx.at(at.b, s) + at.c, C, f);
+            gn_store<V>(dx.at(at.b, s) + at.c, C, at, f);
         }
     }
 }
@@ -466,7 +480,8 @@ static inline GnPlan gn_plan(int B, int S, int C, int G, int bytes) {
 static inline size_t gn_part_bytes(const GnPlan& pl, int B, size_t each) { return align_up((size_t)B * pl.chunks * pl.slices * pl.local * each); }
 static inline size_t gn_ws_bytes(int B, int S, int C, int G, int bytes, bool backward) {
     const GnPlan pl = gn_plan(B, S, C, G, bytes);
-    return backward ? gn_part_bytes(pl, B, sizeof(float2)) + align_up((size_t)B * pl.chunks * 2 * C * sizeof(float)) : gn_part_bytes(pl, B, sizeof(Moments));
+    if (!backward) return gn_part_bytes(pl, B, sizeof(Moments));
+    return gn_part_bytes(pl, B, sizeof(float2)) + align_up((size_t)B * pl.chunks * 2 * C * sizeof(float));
 }
 
 template <class T, int PRE, int POST>
@@ -477,7 +492,8 @@ static int run_group_norm(Rows<const T> x, const float* gamma, const float* beta
     const long grid = (long)B * pl.chunks * pl.slices;
     if (grid > 0x7fffffff) return MSF2_ERR_ARG;
     gn_moments_kernel<T, V, PRE><<<grid, pl.threads, 0, st>>>(x, lengths, (Moments*)ws, pl, S, C);
-    gn_apply_kernel<T, V, PRE, POST><<<grid, pl.threads, pl.local * 2 * sizeof(float), st>>>(x, gamma, beta, lengths, (const Moments*)ws, y, stats, eps, pl, S, C, G);
+    gn_apply_kernel<T, V, PRE, POST>
+        <<<grid, pl.threads, pl.local * 2 * sizeof(float), st>>>(x, gamma, beta, lengths, (const Moments*)ws, y, stats, eps, pl, S, C, G);
     return check_launch();
 }
 
@@ -492,8 +508,8 @@ static int run_group_norm_backward(Rows<const T> dy, Rows<const T> x, const floa
     float2* part = (float2*)ws;
     float* chan = (float*)((char*)ws + gn_part_bytes(pl, B, sizeof(float2)));
     gn_grad_sums_kernel<T, V, PRE, POST><<<grid, pl.threads, 0, st>>>(dy, x, gamma, beta, stats, lengths, chan, part, pl, S, C, G);
-    gn_dx_kernel<T, V, PRE, POST><<<grid + gains, pl.threads, pl.local * 2 * sizeof(float), st>>>(dy, x, gamma, beta, stats, lengths, chan, part, dx, dgamma,
-                                                                                          dbeta, pl, (unsigned)gains, B, S, C, G);
+    gn_dx_kernel<T, V, PRE, POST><<<grid + gains, pl.threads, pl.local * 2 * sizeof(float), st>>>(
+        dy, x, gamma, beta, stats, lengths, chan, part, dx, dgamma, dbeta, pl, (unsigned)gains, B, S, C, G);
     return check_launch();
 }
 

@@ -70,6 +70,9 @@ NORM = [  # B, S, C, groups, type, act, act_first, lengths, strides
     (2, 20, 4100, 1, F32, 1, False, "ends", "plain"),
     (2, 20, 4100, 4100, BF16, 2, False, None, "plain"),     # every channel a group, more of them than a workgroup takes
     (1, 70, 9001, 1, FP16, 0, False, None, "wide"),
+    (1, 20, 65537, 65537, F32, 1, False, None, "plain"),    # the last slice holds one channel, and its lane is moved into the one before
+    (2, 20, 131075, 1, BF16, 0, False, "ends", "plain"),
+    (1, 20, 131078, 65539, FP16, 2, True, None, "plain"),
     (3, 200, 2, 1, BF16, 1, True, "ends", "plain"),         # frames narrower than a vector
     (3, 200, 1, 1, F32, 2, False, None, "wide"),
 ]
