@@ -495,28 +495,44 @@ static inline bool rec_pairs(int bytes, int C, bool backward) { return bytes == 
 // the short form's waves: as many as reach from one saved state to the next
 constexpr int rec_short(int lanes, int rows) { return std::max(1, REC_SAVE / (64 / lanes * rows)); }
 
-// Slices of 256 bytes of a frame where that leaves a workgroup for every CU, else of 128: two lines a row reach 4.9 TB/s, one 4.3
-// (64 x 3999 x 512 bf16 forward: 162 and 184 us).  A sequence is cut into pieces, each read twice, where whole sequences occupy
-// less than 192 of the 256 CUs (16 x 4000 x 512 bf16 forward, 128 workgroups: 58 us in pieces, 74 whole); then into as many as stay
-// on the chip at once, two workgroups a CU forward and, for its registers, one backward (the same case: backward 81 us in 256
-// workgroups, 88 in 512; forward 64 and 58).  Two tiles in a row take less time than another launch does (8.3 and 9.5 us at 4 x 512 x 256
-// fp32), three take more (10.8 and 9.6).
+// The division of the work that takes the least time by this count, in tiles that a CU works off:
+//   whole sequences, workgroups / 256 CUs rounded up;
+//   pieces, where the operands are read twice: 5 / 3 of that forward, or 1.5 with two workgroups on a CU at once, 7 / 5 backward (one
+//   workgroup a CU, for its registers), and another launch, worth 1.5 tiles;
+//   slices of 256 bytes of a frame 0.92 of those of 128 (two lines a row reach 4.9 TB/s, one 4.3).
+// Measured: 16 x 4000 x 512 bf16 forward, 128 sequences, 74 us whole, 58 in 4 pieces, 64 in 2; backward 88 us in 512 workgroups, 81 in
+// 256; 4 x 512 x 256 fp32, two tiles, 8.3 us whole and 9.5 in pieces, three tiles 10.8 and 9.6.
 static inline RecPlan rec_plan(int B, int S, int C, int bytes, bool backward) {
     const int vec = rec_pairs(bytes, C, backward) ? 2 : 8 / bytes, V = C >= vec ? vec : 1, rows = REC_VALUES / vec;
-    RecPlan pl;
-    pl.vec = V;
-    pl.lanes = 256 / (vec * bytes);
-    if (V == 1 || (long)B * ((C + pl.lanes * V - 1) / (pl.lanes * V)) < 256) pl.lanes /= 2;
-    const int wave = 64 / pl.lanes * rows, few = rec_short(pl.lanes, rows);
-    pl.slices = (C + pl.lanes * V - 1) / (pl.lanes * V);
-    pl.waves = S <= few * wave ? few : REC_WIDE;
-    const long tile = (long)pl.waves * wave, tiles = (S + tile - 1) / tile, seqs = (long)B * pl.slices;
-    const long want = seqs >= 192 || tiles <= 2 ? 1 : std::min((backward ? 256 : 512) / seqs, tiles);
-    const long per = (tiles + want - 1) / want;
-    pl.piece = (int)(per * tile);
-    pl.pieces = (int)((tiles + per - 1) / per);
-    pl.near = pl.past = true;
-    return pl;
+    RecPlan best;
+    double least = 0;
+    for (int wide = 1; wide >= 0; --wide) {
+        if (V == 1 && wide) continue;
+        RecPlan pl;
+        pl.vec = V;
+        pl.lanes = (wide ? 256 : 128) / (vec * bytes);
+        const int wave = 64 / pl.lanes * rows, few = rec_short(pl.lanes, rows);
+        pl.slices = (C + pl.lanes * V - 1) / (pl.lanes * V);
+        pl.waves = S <= few * wave ? few : REC_WIDE;
+        const long tile = (long)pl.waves * wave, tiles = (S + tile - 1) / tile, seqs = (long)B * pl.slices;
+        long before = 0;
+        for (int fill = 0; fill <= 8; ++fill) {              // whole, then workgroups for up to 8 times the CUs
+            const long want = fill ? std::min(256l * fill / seqs, tiles) : 1;
+            if (want <= before) continue;
+            before = want;
+            const long per = (tiles + want - 1) / want, pieces = (tiles + per - 1) / per, groups = seqs * pieces;
+            double cost = (double)((groups + 255) / 256 * per);
+            if (pieces > 1) cost = cost * (backward ? 1.4 : groups >= 480 ? 1.5 : 1.67) + 1.5;
+            if (wide) cost *= 0.92;
+            if (least && cost >= least) continue;
+            least = cost;
+            pl.piece = (int)(per * tile);
+            pl.pieces = (int)pieces;
+            best = pl;
+        }
+    }
+    best.near = best.past = true;
+    return best;
 }
 static inline size_t rec_ws_bytes(int B, int S, int C, int bytes, bool backward) {
     const RecPlan pl = rec_plan(B, S, C, bytes, backward);
