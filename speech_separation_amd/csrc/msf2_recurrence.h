@@ -10,7 +10,7 @@
 // lets through to a state that is far smaller.
 // Memory-bound with a busy vector unit (29 instructions a value forward, without its exponential and reciprocal just as fast):
 // 64 x 3999 x 512 bf16 forward 156 us, backward 258 (5.0 and 5.2 TB/s), 16 x 3999 x 512 fp32 83 and 127 us (4.7 and 5.3), one sequence
-// of 61499 x 512 bf16 in pieces 28 + 39 us.
+// of 61499 x 512 bf16 in pieces 25 + 38 us.
 // t counts frames in walking order; frame s is t, or S - 1 - t in reverse.  Frames past an utterance's end count as a = 1, B = 0.
 #pragma once
 #include <algorithm>

@@ -232,6 +232,11 @@ def _out_rows(t, name, like, same_type=True, apart=(), same=()):
     return r
 
 
+def _new(x):
+    """A contiguous tensor of x's shape and type (empty_like is the quicker call, but keeps other strides)."""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 def _written(*ts):
     """Tensors of the caller's that a kernel is about to write: autograd is told, as by any operation in place."""
     for t in ts:
@@ -278,7 +283,7 @@ def group_norm_act(x, gamma, beta, groups, eps=1e-5, act=_lib.ACT_NONE, act_firs
         raise ValueError(f"unknown activation {act}")
     dev = x.device
     side = (_aside(gamma, "gamma", (C,), dev), _aside(beta, "beta", (C,), dev), _aside(lengths, "lengths", (B,), dev, torch.int32))
-    y = torch.empty((B, S, C), dtype=x.dtype, device=dev)
+    y = _new(x)
     if not (B and S):
         return y, torch.zeros((B, groups, 2), device=dev)
     stats = torch.empty((B, groups, 2), device=dev)
@@ -303,7 +308,7 @@ def group_norm_act_backward(dy, x, gamma, beta, stats, groups, act=_lib.ACT_NONE
             _aside(lengths, "lengths", (B,), dev, torch.int32))
     if side[2] is None:
         raise ValueError("stats: expected what group_norm_act returned")
-    dx = torch.empty((B, S, C), dtype=x.dtype, device=dev)
+    dx = _new(x)
     new = torch.empty if B and S else torch.zeros
     dgamma = None if gamma is None else new((C,), device=dev)
     dbeta = None if beta is None else new((C,), device=dev)
@@ -336,7 +341,7 @@ def gated_recurrence(x, gate, h0=None, lengths=None, reverse=False, last=None, s
         if any(u is not None and _clash(last, u) for u in (x, gate)) or (h0 is not None and _clash(last, h0) and lastp != h0p):
             raise ValueError("last: the output shares memory with another operand")
         _written(last)
-    h = torch.empty((B, S, C), dtype=x.dtype, device=dev)
+    h = _new(x)
     saved = torch.empty((B, -(-S // _lib.RECURRENCE_SAVE), C), device=dev) if save else None
     if B and S:
         t = _TYPES[x.dtype]
@@ -360,7 +365,7 @@ def gated_recurrence_backward(dh, x, gate, saved, dlast=None, lengths=None, reve
         raise ValueError("x has no channels")
     dev = x.device
     if out is None:
-        dx, dgate = (torch.empty((B, S, C), dtype=x.dtype, device=dev) for _ in range(2))
+        dx, dgate = _new(x), _new(x)
         dxr, dgr = (dx.data_ptr(), S * C, C), (dgate.data_ptr(), S * C, C)
     else:
         dx, dgate = out
@@ -414,7 +419,9 @@ def dropout(x, p, rng, site=0, residual=None, out=None):
         yr = _out_rows(out, "out", x, same_type=False, apart=(rng,), same=(x, residual))
         _written(out)
         return _dropout(x, p, rng, site, residual, out, yr)
-    return _dropout(x, p, rng, site, residual, torch.empty(x.shape, dtype=(x if residual is None else residual).dtype, device=x.device))
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"residual: expected shape {tuple(x.shape)}, got {tuple(residual.shape)}")
+    return _dropout(x, p, rng, site, residual, _new(x if residual is None else residual))
 
 
 def dropout_backward(dy, p, rng, site=0, dtype=None):
@@ -422,4 +429,5 @@ def dropout_backward(dy, p, rng, site=0, dtype=None):
     the forward's p, rng and site.  The residual's gradient is dy itself."""
     if not isinstance(dy, torch.Tensor):
         raise ValueError("dy: expected a tensor")
-    return _dropout(dy, p, rng, site, None, torch.empty(dy.shape, dtype=dtype or dy.dtype, device=dy.device))
+    dx = _new(dy) if dtype in (None, dy.dtype) else torch.empty(dy.shape, dtype=dtype, device=dy.device)
+    return _dropout(dy, p, rng, site, None, dx)

@@ -289,6 +289,25 @@ def test_gated_recurrence_gradients_into_one_tensor():
     assert bool((d[..., 0] == 7).all()) and bool((d[..., 81:] == 7).all())
 
 
+@pytest.mark.parametrize("S,C,dtype", [(50, 33, F32), (3000, 131, F32), (3000, 66, BF16)])
+def test_gated_recurrence_keeps_a_bad_value_in_its_channel(S, C, dtype):
+    """Not a number from one frame on in the channels it came in by, forward and backward, and nowhere else."""
+    g = torch.Generator().manual_seed(16)
+    x, gate, dh, _, _ = rec_inputs(g, 2, S, C, dtype, None)
+    x[0, 7, C - 1], gate[1, 20, 3], dh[0, S - 9, 0] = NAN, NAN, NAN
+    xd, gd, dhd = to_dev(x, gate, dh)
+    h, last, saved = ops.gated_recurrence(xd, gd, save=True)
+    want = torch.zeros(2, S, C, dtype=torch.bool)
+    want[0, 7:, C - 1] = want[1, 20:, 3] = True
+    assert torch.equal(torch.isnan(h).cpu(), want) and torch.equal(torch.isnan(last).cpu(), want[:, -1])
+    dx, dgate, dh0 = ops.gated_recurrence_backward(dhd, xd, gd, saved)
+    back = torch.zeros(2, S, C, dtype=torch.bool)
+    back[0, :S - 8, 0] = back[1, :21, 3] = True
+    assert torch.equal(torch.isnan(dx).cpu(), back)
+    back[0, 7:, C - 1] = back[1, 20:, 3] = True              # h_{t-1} - x_t
+    assert torch.equal(torch.isnan(dgate).cpu(), back) and bool(torch.isnan(dh0[0, 0])) and int(torch.isnan(dh0).sum()) == 2
+
+
 def test_gated_recurrence_empty():
     for B, S in ((0, 4), (3, 0)):
         x = torch.zeros(B, S, 8, device=DEV)
