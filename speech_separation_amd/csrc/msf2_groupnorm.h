@@ -13,9 +13,10 @@
 // next call then find no results to write back, 48 us instead of 72).  A read from that cache is not much faster than one from memory
 // (5.9 and 5.2 TB/s), so walking a batch in parts that fit it was no gain.
 //
-// Statistics: each thread sums (u - K) and (u - K)^2 over its frames in 32 bits, K the first value that its channel has in the
-// chunk, so a mean far from zero costs no digits of the variance; what lies above a channel is joined as
-// (count, mean, sum of squared deviations).
+// Statistics: each thread sums u - K and (u - K)^2 over its frames, 64 at most, in 32 bits, K the first of its own values.  So a mean far
+// from zero costs no digits of the variance, and an untypical K is that of one thread: as K is among the n values, the
+// squares sum to no more than n times their squared deviations from the mean.  From there on everything is joined in 64 bits as (count,
+// mean, sum of squared deviations); a K for the whole chunk and 32-bit joins lost 2.5 % of a variance to one frame.
 #pragma once
 #include <algorithm>
 #include "msf2_rows.h"
@@ -30,7 +31,7 @@ constexpr int GN_ROWS = 64;                  // frames a thread sums in 32 bits 
 // group counts from the first that touches it; at most `local` groups do.
 struct GnPlan {
     int lanes, step, threads, width, slices, chunks, rows, local, D;     // step: frames that a workgroup takes side by side
-    Divider by_D, by_width;
+    Divider by_D, by_width, by_step;
     __device__ int group(int c) const { return by_D.div(c); }
     __device__ int first(int slice) const { return group(slice * width); }
     __device__ int last(int slice, int C) const { return group(min((slice + 1) * width, C) - 1); }
@@ -113,11 +114,6 @@ template <int V> __device__ __forceinline__ void gn_note(float* table, const GnP
         if (v >= at.own) p[v] = f[v];
 }
 
-template <int J> __device__ __forceinline__ float sum_lanes(float v) {
-#pragma unroll
-    for (int o = 1; o < J; o *= 2) v += __shfl_xor(v, o, 64);
-    return v;
-}
 template <int J> __device__ __forceinline__ double sum_lanes(double v) {
 #pragma unroll
     for (int o = 1; o < J; o *= 2) v += __shfl_xor(v, o, 64);
@@ -128,6 +124,15 @@ template <class F> __device__ __forceinline__ void gn_spread(int groups, F f) {
     if (groups <= (int)blockDim.x / 64) f(std::integral_constant<int, 64>());
     else if (groups <= (int)blockDim.x / 32) f(std::integral_constant<int, 32>());
     else f(std::integral_constant<int, 16>());
+}
+
+// f(J) with J neighbouring lanes a channel of a slice w wide: narrow frames are many side by side, and so a channel's sums are 32 at most
+// for a lane.
+template <class F> __device__ __forceinline__ void gn_columns(int w, F f) {
+    if (w > (int)blockDim.x / 4) f(std::integral_constant<int, 1>());
+    else if (w > (int)blockDim.x / 16) f(std::integral_constant<int, 4>());
+    else if (w > (int)blockDim.x / 64) f(std::integral_constant<int, 16>());
+    else f(std::integral_constant<int, 64>());
 }
 
 // Every group that touches a slice, J threads each: f(g, j, each), where each(h) calls h on the group's sums over all
@@ -155,7 +160,9 @@ __global__ __launch_bounds__(GN_T) void gn_moments_kernel(Rows<const T> x, const
     __shared__ float s_s[GN_T * V], q_s[GN_T * V];
     const GnPlace<V> at(pl, blockIdx.x, C);
     const int n = frames_of(lengths, at.b, S), s0 = at.chunk * pl.rows, s1 = min(s0 + pl.rows, n), c0 = at.slice * pl.width;
-    typename VecOf<T, V>::type u[U], k;
+    const unsigned count = max(s1 - s0, 0), rounds = pl.by_step.div(count), more = count - rounds * at.step;
+    auto frames = [&](int r0) { return rounds + ((unsigned)r0 < more); };       // of the threads r0 of the workgroup
+    typename VecOf<T, V>::type u[U];
     const bool some = at.have > 0 && s0 + at.r0 < s1;
     auto fetch = [&](int r) {
 #pragma unroll
@@ -165,10 +172,9 @@ __global__ __launch_bounds__(GN_T) void gn_moments_kernel(Rows<const T> x, const
 #pragma unroll
     for (int v = 0; v < V; ++v) s[v] = q[v] = 0.f;
     if (some) {
-        k = gn_load<V>(x.at(at.b, s0) + at.c, C);
         fetch(s0 + at.r0);
 #pragma unroll
-        for (int v = 0; v < V; ++v) K[v] = act_f<PRE, fine<T>()>((float)k[v]);
+        for (int v = 0; v < V; ++v) K[v] = act_f<PRE, fine<T>()>((float)u[0][v]);
         for (int r = s0 + at.r0; r < s1; r += U * at.step) {
             typename VecOf<T, V>::type w[U];
 #pragma unroll
@@ -186,19 +192,41 @@ __global__ __launch_bounds__(GN_T) void gn_moments_kernel(Rows<const T> x, const
             }
         }
     }
+    if (some) {                              // s becomes the mean, q the squared deviations from it; not a number stays one
+        const float inv = 1.f / (float)frames(at.r0);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const float m = fmaf(-s[v] * inv, s[v], q[v]);
+            q[v] = m < 0.f ? 0.f : m;
+            s[v] = fmaf(s[v], inv, K[v]);
+        }
+    }
     gn_note<V>(s_s, pl, at, s);
     gn_note<V>(q_s, pl, at, q);
     __syncthreads();
-    // a channel's frames together: (mean, M2) over the chunk; this thread alone reads and writes column i
+    // a channel's frames together: (mean, squared deviations) over the chunk; the J lanes of column i alone read and write it
     const int w = min(pl.width, C - c0);
-    const float count = (float)max(s1 - s0, 0), inv = count > 0.f ? 1.f / count : 0.f;
-    for (int i = threadIdx.x; i < w; i += blockDim.x) {
-        float p = 0.f, m = 0.f;
-        for (int k = 0; k < at.step; ++k) p += s_s[k * pl.width + i], m += q_s[k * pl.width + i];
-        const float first = count > 0.f ? act_f<PRE, fine<T>()>((float)x.at(at.b, s0)[c0 + i]) : 0.f;
-        s_s[i] = fmaf(p, inv, first);
-        q_s[i] = fmaxf(fmaf(-p * inv, p, m), 0.f) + (m - m);         // not a number stays one
-    }
+    gn_columns(count ? w : 0, [&](auto jj) {
+        constexpr int J = decltype(jj)::value;
+        const int j = threadIdx.x % J;
+        const double inv = 1. / count;
+        for (int i = threadIdx.x / J; i < (count ? w : 0); i += blockDim.x / J) {
+            const double first = s_s[i];
+            double p = 0, m = 0;
+            for (int k = j; k < at.step; k += J) {
+                const double d = s_s[k * pl.width + i] - first, n = frames(k);
+                p += n * d;
+                m += q_s[k * pl.width + i] + n * d * d;
+            }
+            p = sum_lanes<J>(p);
+            m = sum_lanes<J>(m);
+            m -= p * inv * p;
+            if (j == 0) {
+                s_s[i] = (float)(first + p * inv);
+                q_s[i] = m < 0 ? 0.f : (float)m;
+            }
+        }
+    });
     __syncthreads();
     const int g0 = pl.first(at.slice), groups = pl.last(at.slice, C) - g0 + 1;
     Moments* out = part + (((long)at.b * pl.chunks + at.chunk) * pl.slices + at.slice) * pl.local;
@@ -207,12 +235,12 @@ __global__ __launch_bounds__(GN_T) void gn_moments_kernel(Rows<const T> x, const
         const int j = threadIdx.x % J;
         for (int g = threadIdx.x / J; g < groups; g += blockDim.x / J) {
             const int w0 = max((g0 + g) * pl.D - c0, 0), w1 = min((g0 + g + 1) * pl.D - c0, w);
-            float mean = 0.f, m2 = 0.f;
+            double mean = 0, m2 = 0;
             for (int i = w0 + j; i < w1; i += J) mean += s_s[i];
-            mean = sum_lanes<J>(mean) / (float)(w1 - w0);
-            for (int i = w0 + j; i < w1; i += J) m2 += fmaf(count * (s_s[i] - mean), s_s[i] - mean, q_s[i]);
+            mean = sum_lanes<J>(mean) / (w1 - w0);
+            for (int i = w0 + j; i < w1; i += J) m2 += (double)count * (s_s[i] - mean) * (s_s[i] - mean) + q_s[i];
             m2 = sum_lanes<J>(m2);
-            if (j == 0) out[g] = {count * (float)(w1 - w0), mean, m2};
+            if (j == 0) out[g] = {(float)count * (float)(w1 - w0), (float)mean, (float)m2};
         }
     });
 }
@@ -340,15 +368,23 @@ __global__ __launch_bounds__(GN_T) void gn_grad_sums_kernel(Rows<const T> dy, Ro
     __syncthreads();
     const int w = min(pl.width, C - c0);
     float* out = chan + ((long)at.b * pl.chunks + at.chunk) * 2 * C + c0;
-    for (int i = threadIdx.x; i < w; i += blockDim.x) {
-        float p = 0.f, q = 0.f;
-        for (int k = 0; k < at.step; ++k) p += s1_s[k * pl.width + i], q += s2_s[k * pl.width + i];
-        out[i] = p;
-        out[C + i] = q;
-        const float k = gamma ? gamma[c0 + i] : 1.f;
-        s1_s[i] = p * k;                     // this thread alone reads column i
-        s2_s[i] = q * k;
-    }
+    gn_columns(w, [&](auto jj) {
+        constexpr int J = decltype(jj)::value;
+        const int j = threadIdx.x % J;
+        for (int i = threadIdx.x / J; i < w; i += blockDim.x / J) {
+            double p = 0, q = 0;
+            for (int k = j; k < at.step; k += J) p += s1_s[k * pl.width + i], q += s2_s[k * pl.width + i];
+            p = sum_lanes<J>(p);
+            q = sum_lanes<J>(q);
+            if (j == 0) {
+                out[i] = (float)p;
+                out[C + i] = (float)q;
+                const float k = gamma ? gamma[c0 + i] : 1.f;
+                s1_s[i] = (float)p * k;      // the J lanes of column i alone read it
+                s2_s[i] = (float)q * k;
+            }
+        }
+    });
     __syncthreads();
     const int g0 = pl.first(at.slice), groups = pl.last(at.slice, C) - g0 + 1;
     gn_spread(groups, [&](auto jj) {
@@ -356,11 +392,11 @@ __global__ __launch_bounds__(GN_T) void gn_grad_sums_kernel(Rows<const T> dy, Ro
         const int j = threadIdx.x % J;
         for (int g = threadIdx.x / J; g < groups; g += blockDim.x / J) {
             const int w0 = max((g0 + g) * pl.D - c0, 0), w1 = min((g0 + g + 1) * pl.D - c0, w);
-            float p = 0.f, q = 0.f;
+            double p = 0, q = 0;
             for (int i = w0 + j; i < w1; i += J) p += s1_s[i], q += s2_s[i];
             p = sum_lanes<J>(p);
             q = sum_lanes<J>(q);
-            if (j == 0) part[(((long)at.b * pl.chunks + at.chunk) * pl.slices + at.slice) * pl.local + g] = make_float2(p, q);
+            if (j == 0) part[(((long)at.b * pl.chunks + at.chunk) * pl.slices + at.slice) * pl.local + g] = make_float2((float)p, (float)q);
         }
     });
 }
@@ -467,6 +503,7 @@ static inline GnPlan gn_plan(int B, int S, int C, int G, int bytes) {
     auto idle = [&](int step) { const int t = step * pl.lanes; return 1. - (double)t / ((t + 63) / 64 * 64); };
     if (idle(512 / pl.lanes) + 0.05 < idle(pl.step)) pl.step = 512 / pl.lanes;
     pl.threads = (pl.step * pl.lanes + 63) / 64 * 64;
+    pl.by_step = Divider(pl.step);
     pl.width = pl.lanes * V;
     pl.by_width = Divider(pl.width);
     pl.slices = (vecs + pl.lanes - 1) / pl.lanes;

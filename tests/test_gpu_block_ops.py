@@ -663,3 +663,45 @@ def _tail_keep(S, C, rows):
     block = np.arange((S - rows) * per, S * per, dtype=np.uint64)
     w = oracle.philox([block & np.uint64(0xFFFFFFFF), block >> np.uint64(32), np.full_like(block, 4), np.full_like(block, 5)], [3, 0])
     return np.stack(w, -1).astype("<u4").view("<u2").reshape(rows, per * 8)[:, :C] >= 16384
+
+
+# A thread sums n <= 64 values of one channel about the first of them, K: d = u - K, s = sum d, q = sum d^2, M2 = q - s^2 / n.  In 32
+# bits q is off by (n + 2) U q and s by n U sum |d|, which changes s^2 / n by 2 n U q at most (|s| sum |d| <= n q); so M2 is off by
+# (3 n + 4) U q.  K is one of the values, so (K - mean)^2 <= M2 (n - 1) / n and q = M2 + n (K - mean)^2 <= n M2.  The thread's mean is
+# off by e = U sum |d| <= U sqrt(n q), and that of all values by the sum of 2 n e |its mean - theirs| more: by Cauchy, with M2 of all
+# of them, 2 U n sqrt(n) M2 at most.
+NORM_M2 = ((3 * 64 + 4) * 64 + 2 * 64 * 8) * oracle.U
+
+
+@pytest.mark.parametrize("B,S,C,dtype,first", [(257, 16384, 4, F32, 1000.0), (257, 16384, 8, BF16, 1000.0), (300, 4096, 64, F32, -3000.0), (2, 4000, 512, F32, 1000.0)])
+def test_group_norm_act_outlying_first_frame(B, S, C, dtype, first):
+    """One frame unlike all others at the head of every utterance, in chunks of thousands of frames: it costs no digits of the variance."""
+    g = torch.Generator(device=DEV).manual_seed(61)
+    x = torch.randn(B, S, C, generator=g, device=DEV)
+    x[:, 0] = first
+    x = x.to(dtype)
+    _, stats = ops.group_norm_act(x, None, None, 1)
+    for b in range(0, B, 50):
+        v = x[b].double()
+        mean, var = v.mean(), v.var(unbiased=False)
+        # a channel's, a thread's and the group's mean are rounded to 32 bits: 3 U of the largest each, twice as a factor of a deviation
+        m = float(v.abs().mean())
+        assert abs(float(stats[b, 0, 0]) - float(mean)) <= 70 * oracle.U * (m + abs(float(mean)) + float(var) ** 0.5)
+        got = float(stats[b, 0, 1].double() ** -2 - 1e-5)
+        assert abs(got / float(var) - 1) <= NORM_M2 + 16 * oracle.U, (b, got, float(var))
+
+
+def test_group_norm_act_sums_of_many_threads():
+    """Narrow frames, whose channels are summed by 256 threads: one large sum first, then 255 of less than half its last bit each.  No
+    more than 64 terms are added one after the other in 32 bits, so no sum is off by more than 64 U of its terms."""
+    S, C = 1024, 4
+    many = torch.zeros(1, S, C, device=DEV)
+    many[0, 1], many[0, 2:256] = 2.0 ** 24, 1.0
+    total = 2.0 ** 24 + 254
+    _, stats = ops.group_norm_act(many, None, None, 1)
+    assert abs(float(stats[0, 0, 0]) - total / S) <= 65 * oracle.U * total / S
+    x = torch.randn(1, S, C, device=DEV)
+    w = torch.ones(C, device=DEV)
+    _, stats = ops.group_norm_act(x, w, w, 1)
+    _, _, dbeta = ops.group_norm_act_backward(many, x, w, w, stats, 1)
+    assert bool(((dbeta.double() - total).abs() <= 65 * oracle.U * total).all()), dbeta
