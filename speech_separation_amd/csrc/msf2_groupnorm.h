@@ -58,6 +58,10 @@ template <int V> struct GnPlace {
     }
 };
 
+// z from a deviation from the mean, ga = gamma rstd: the same expression in every pass, so that the gradient of a ReLU is that of the
+// side of zero on which its result was.
+__device__ __forceinline__ float gn_affine(float dev, float ga, float be) { return fmaf(dev, ga, be); }
+
 struct Moments {
     float n, mean, m2;
 };
@@ -309,7 +313,7 @@ __global__ __launch_bounds__(GN_T) void gn_apply_kernel(Rows<const T> x, const f
             float f[V];
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                f[v] = act_f<POST, fine<T>()>(fmaf(act_f<PRE, fine<T>()>((float)w[j][v]) - mean[v], ga[v], be[v]));
+                f[v] = act_f<POST, fine<T>()>(gn_affine(act_f<PRE, fine<T>()>((float)w[j][v]) - mean[v], ga[v], be[v]));
                 if (s >= n) f[v] = 0.f;
             }
             gn_store<V>(y.at(at.b, s) + at.c, C, at, f);
@@ -344,7 +348,7 @@ __global__ __launch_bounds__(GN_T) void gn_grad_sums_kernel(Rows<const T> dy, Ro
     gn_channels<V>(gamma, at.c, C, 1.f, ga);
     gn_channels<V>(beta, at.c, C, 0.f, be);
 #pragma unroll
-    for (int v = 0; v < V; ++v) a1[v] = a2[v] = 0.f;
+    for (int v = 0; v < V; ++v) a1[v] = a2[v] = 0.f, ga[v] *= rstd[v];
     if (some)
         for (int r = s0 + at.r0; r < s1; r += U * at.step) {
             typename VecOf<T, V>::type w[U], e[U];
@@ -356,10 +360,10 @@ __global__ __launch_bounds__(GN_T) void gn_grad_sums_kernel(Rows<const T> dy, Ro
                 if (r + j * at.step >= s1) break;
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    const float xh = (act_f<PRE, fine<T>()>((float)w[j][v]) - mean[v]) * rstd[v];
-                    const float dz = (float)e[j][v] * act_grad_f<POST, fine<T>()>(fmaf(xh, ga[v], be[v]));
+                    const float dev = act_f<PRE, fine<T>()>((float)w[j][v]) - mean[v];
+                    const float dz = (float)e[j][v] * act_grad_f<POST, fine<T>()>(gn_affine(dev, ga[v], be[v]));
                     a1[v] += dz;
-                    a2[v] = fmaf(dz, xh, a2[v]);
+                    a2[v] = fmaf(dz, dev * rstd[v], a2[v]);
                 }
             }
         }
@@ -466,6 +470,8 @@ __global__ __launch_bounds__(GN_T) void gn_dx_kernel(Rows<const T> dy, Rows<cons
     gn_of_groups<V>(st, g0, pl, at.c, C, c1, c2);
     gn_channels<V>(gamma, at.c, C, 1.f, ga);
     gn_channels<V>(beta, at.c, C, 0.f, be);
+#pragma unroll
+    for (int v = 0; v < V; ++v) ga[v] *= rstd[v], c1[v] *= rstd[v], c2[v] *= rstd[v];
     for (int r = s0 + at.r0; r < s1; r += U * at.step) {
         typename VecOf<T, V>::type w[U], e[U];
 #pragma unroll
@@ -478,9 +484,9 @@ __global__ __launch_bounds__(GN_T) void gn_dx_kernel(Rows<const T> dy, Rows<cons
             float f[V];
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const float xv = (float)w[j][v], xh = (act_f<PRE, fine<T>()>(xv) - mean[v]) * rstd[v];
-                const float dz = (float)e[j][v] * act_grad_f<POST, fine<T>()>(fmaf(xh, ga[v], be[v]));
-                f[v] = rstd[v] * (fmaf(dz, ga[v], -c1[v]) - xh * c2[v]) * act_grad_f<PRE, fine<T>()>(xv);
+                const float xv = (float)w[j][v], dev = act_f<PRE, fine<T>()>(xv) - mean[v];
+                const float dz = (float)e[j][v] * act_grad_f<POST, fine<T>()>(gn_affine(dev, ga[v], be[v]));
+                f[v] = (fmaf(dz, ga[v], -c1[v]) - dev * rstd[v] * c2[v]) * act_grad_f<PRE, fine<T>()>(xv);
                 if (s >= n) f[v] = 0.f;
             }
             gn_store<V>(dx.at(at.b, s) + at.c, C, at, f);

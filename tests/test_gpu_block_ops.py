@@ -705,3 +705,25 @@ def test_group_norm_act_sums_of_many_threads():
     _, stats = ops.group_norm_act(x, w, w, 1)
     _, _, dbeta = ops.group_norm_act_backward(many, x, w, w, stats, 1)
     assert bool(((dbeta.double() - total).abs() <= 65 * oracle.U * total).all()), dbeta
+
+
+@pytest.mark.parametrize("C,G", [(512, 512), (131, 131), (256, 32)])
+def test_group_norm_relu_gradient_goes_by_the_forward(C, G):
+    """Values within roundings of the corner of a ReLU: the gradient passes exactly where the forward's result is above zero."""
+    B, S = 1, 64
+    g = torch.Generator().manual_seed(62)
+    x, gamma = randn(g, B, S, C).to(DEV), (1 + 0.2 * randn(g, C)).to(DEV)
+    _, stats = ops.group_norm_act(x, None, None, G)
+    mean, rstd = (stats[0, :, k].repeat_interleave(C // G) for k in (0, 1))
+    at = torch.arange(C, device=DEV) % S                    # the frame of channel c that beta moves to the corner
+    c = torch.arange(C, device=DEV)
+    beta = -((x[0, at, c] - mean) * rstd * gamma)
+    y, stats = ops.group_norm_act(x, gamma, beta, G, act=_lib.ACT_RELU)
+    above = y[0, at, c] > 0
+    assert 0 < int(above.sum()) < C                         # of such values some lie on either side
+    dy = torch.zeros_like(x)
+    dy[0, at, c] = 1.0
+    dx, _, dbeta = ops.group_norm_act_backward(dy, x, gamma, beta, stats, G, act=_lib.ACT_RELU)
+    assert torch.equal(dbeta, above.float())
+    if C == G:                                              # a channel that lets nothing through has no gradient anywhere
+        assert torch.equal((dx[0] != 0).any(0), above)
