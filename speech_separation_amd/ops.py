@@ -203,16 +203,28 @@ def _span(t):
     return t.data_ptr(), t.data_ptr() + n * t.element_size()
 
 
+def _meets(off, axes):
+    """Whether off = sum d_i stride_i with |d_i| < size_i, axes = (stride, size) from the widest stride down.  Of a tensor whose
+    elements do not share addresses the rest reaches less than a stride, so three steps of an axis are tried at most."""
+    if not axes:
+        return off == 0
+    (st, n), rest = axes[0], axes[1:]
+    reach = sum((k - 1) * t for t, k in rest)
+    if st == 0:
+        return _meets(off, rest)
+    return any(_meets(off - d * st, rest) for d in range(max(1 - n, -((reach - off) // st)), min(n - 1, (off + reach) // st) + 1))
+
+
 def _clash(t, u):
-    """Whether two tensors share memory.  Interleaved ones (two halves of one wider tensor) do not."""
+    """Whether two tensors share memory.  Those of one shape and the same strides (those of one-element dimensions aside) are
+    compared element by element, so parts of one larger tensor are told apart however it is laid out."""
     (a, b), (c, d) = _span(t), _span(u)
     if b <= c or d <= a or a == b or c == d:
         return False
-    if t.dim() == 3 and t.shape == u.shape and t.stride() == u.stride() and t.element_size() == u.element_size():
-        C, row, e = t.shape[2], t.stride(1), t.element_size()
-        if t.shape[0] > 1 and t.stride(0) % max(row, 1):
-            return True
-        return (c - a) % e != 0 or not C <= (c - a) // e % max(row, 1) <= row - C
+    e = t.element_size()
+    axes = [sorted(((st, n) for st, n in zip(v.stride(), v.shape) if n > 1), reverse=True) for v in (t, u)]
+    if t.shape == u.shape and axes[0] == axes[1] and e == u.element_size() and (c - a) % e == 0:
+        return _meets((c - a) // e, axes[0])
     return True
 
 

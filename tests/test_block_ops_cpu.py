@@ -148,3 +148,39 @@ def test_oracle_keep_rate():
         sigma = (p * (1 - p) / k.numel()) ** 0.5
         assert abs(float(k.mean()) - (1 - p)) < 5 * sigma
     assert np.array_equal(oracle.keep((1, 6, 17), 0.3, 1, 2, 3)[0, 3:].numpy(), oracle.keep((2, 3, 17), 0.3, 1, 2, 3)[1].numpy())
+
+
+def test_overlap_check_of_other_layouts():
+    """Frame-major halves, one-frame halves whose unused strides differ, frames before and behind one another: apart; a part of any of them
+    moved by less than its own width, or onto itself: not."""
+    turned = torch.zeros(5, 4, 35).transpose(0, 1)                       # [S, B, C] in memory
+    x, g = turned[..., :16], turned[..., 16:32]
+    assert not ops._clash(x, g) and not ops._clash(g, x)
+    assert ops._clash(x, x) and ops._clash(x, turned[..., 15:31]) and ops._clash(turned[..., 17:33], g) and ops._clash(turned, turned)
+    assert not ops._clash(turned[:, :2], turned[:, 2:4]) and not ops._clash(turned[:2], turned[2:]) and ops._clash(turned[:, 1:], turned[:, :-1])
+    assert ops._clash(turned[:3, :, :16], turned[1:, :, 10:26]) and not ops._clash(turned[:3, :, :16], turned[1:, :, 16:32])
+    one = torch.zeros(4, 1, 32)
+    x, g = one[..., :16].as_strided((4, 1, 16), (32, 7, 1)), one[..., 16:]
+    assert not ops._clash(x, g) and not ops._clash(g, x) and ops._clash(x, one[..., :16]) and ops._clash(x, one[..., 3:19])
+    both = torch.zeros(3, 10, 8)
+    assert not ops._clash(both[:, :5], both[:, 5:]) and ops._clash(both[:, :6], both[:, 4:])
+    one = torch.zeros(3, 10, 2)
+    assert not ops._clash(one[..., :1], one[..., 1:]) and ops._clash(one[..., :1], one[..., :1])
+
+
+def test_overlap_check_agrees_with_the_addresses():
+    rng = np.random.default_rng(63)
+    n = 0
+    for _ in range(3000):
+        B, S, C = (int(v) for v in rng.integers(1, 5, 3))
+        order = rng.permutation(2)
+        inner = C + int(rng.integers(0, 4))
+        st = [0, 0]
+        st[order[0]] = inner
+        st[order[1]] = inner * (S if order[0] else B) + int(rng.integers(0, 7))
+        base = torch.zeros(400)
+        t, u = (base.as_strided((B, S, C), (st[0], st[1], 1), int(rng.integers(0, 60))) for _ in range(2))
+        at = [{int(v.storage_offset() + b * st[0] + s * st[1] + c) for b in range(B) for s in range(S) for c in range(C)} for v in (t, u)]
+        assert ops._clash(t, u) == bool(at[0] & at[1]), (B, S, C, st, t.storage_offset(), u.storage_offset())
+        n += bool(at[0] & at[1])
+    assert 500 < n < 2500

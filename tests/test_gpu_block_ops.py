@@ -727,3 +727,21 @@ def test_group_norm_relu_gradient_goes_by_the_forward(C, G):
     assert torch.equal(dbeta, above.float())
     if C == G:                                              # a channel that lets nothing through has no gradient anywhere
         assert torch.equal((dx[0] != 0).any(0), above)
+
+
+def test_outputs_into_parts_of_frame_major_and_one_frame_tensors():
+    g = torch.Generator().manual_seed(64)
+    for B, S in ((3, 200), (5, 1)):
+        both = randn(g, S, B, 80, dtype=BF16).to(DEV).transpose(0, 1)
+        x, gate, dh = both[..., :40], both[..., 40:], place(randn(g, B, S, 40, dtype=BF16), "frames")
+        _, _, saved = ops.gated_recurrence(x, gate, save=True)
+        want = ops.gated_recurrence_backward(dh, x, gate, saved)
+        d = torch.full((S, B, 83), 7.0, dtype=BF16, device=DEV).transpose(0, 1)
+        dh0 = ops.gated_recurrence_backward(dh, x, gate, saved, out=(d[..., 1:41], d[..., 41:81]))[2]
+        assert torch.equal(d[..., 1:41], want[0]) and torch.equal(d[..., 41:81], want[1]) and torch.equal(dh0, want[2])
+        assert bool((d[..., 0] == 7).all()) and bool((d[..., 81:] == 7).all())
+        rng = torch.tensor([5, 6], device=DEV)
+        drop = ops.dropout(x, 0.2, rng, 4, gate)
+        assert ops.dropout(x, 0.2, rng, 4, gate, out=gate) is gate and torch.equal(both[..., 40:], drop)
+        with pytest.raises(ValueError):
+            ops.dropout(x, 0.2, rng, 4, out=both[..., 20:60])
