@@ -338,7 +338,9 @@ int msf2_pit_si_snr_noalloc(const float* est, const float* src, float* si_snr, f
  * as one projection writes them).  No alignment beyond the element's is asked for.  Arithmetic, statistics, states and
  * sums are fp32 or wider whatever the element type.  Outputs must not overlap inputs, except where stated.
  * `lengths` (int32 [B] on the device, or null: all S): frames at and past lengths[b] belong to no utterance.  They are not
- * read into any result, whatever they hold, and outputs are zero there.  Values outside [0, S] count as the nearer end. */
+ * read into any result, whatever they hold, and outputs are zero there.  Values outside [0, S] count as the nearer end.
+ * S and C are below 2^30 and B S C is at most 2^46; a call whose launch would take 2^32 threads or more (from 2^24 utterances of a frame
+ * in the norm, 2^25 in the recurrence) is refused: MSF2_ERR_ARG. */
 #define MSF2_TYPE_FP32 0
 #define MSF2_TYPE_BF16 1
 #define MSF2_TYPE_FP16 2

@@ -8,8 +8,10 @@
 
 using namespace msf2;
 
-// S below 2^30: frame indices, and the end of the tile that holds the last one, stay below 2^31
-static inline bool sizes_ok(int B, int S, int C) { return B >= 1 && S >= 1 && S < 1 << 30 && C >= 1 && (long)B * S <= (1l << 46) / C; }
+// S and C below 2^30: indices of frames and channels, and the end of the tile that holds the last one, stay below 2^31
+static inline bool sizes_ok(int B, int S, int C) {
+    return B >= 1 && S >= 1 && S < 1 << 30 && C >= 1 && C < 1 << 30 && (long)B * S <= (1l << 46) / C;
+}
 static inline bool type_ok(int type) { return type == MSF2_TYPE_FP32 || type == MSF2_TYPE_BF16 || type == MSF2_TYPE_FP16; }
 static inline int type_bytes(int type) { return type == MSF2_TYPE_FP32 ? 4 : 2; }
 static inline bool norm_ok(int B, int S, int C, int groups, int type) {

@@ -536,7 +536,7 @@ static int run_group_norm(Rows<const T> x, const float* gamma, const float* beta
     constexpr int V = gn_vec(sizeof(T));
     const GnPlan pl = gn_plan(B, S, C, G, sizeof(T));
     const long grid = (long)B * pl.chunks * pl.slices;
-    if (grid > 0x7fffffff) return MSF2_ERR_ARG;
+    if (!launch_ok(grid, pl.threads)) return MSF2_ERR_ARG;
     gn_moments_kernel<T, V, PRE><<<grid, pl.threads, 0, st>>>(x, lengths, (Moments*)ws, pl, S, C);
     gn_apply_kernel<T, V, PRE, POST>
         <<<grid, pl.threads, pl.local * 2 * sizeof(float), st>>>(x, gamma, beta, lengths, (const Moments*)ws, y, stats, eps, pl, S, C, G);
@@ -550,7 +550,7 @@ static int run_group_norm_backward(Rows<const T> dy, Rows<const T> x, const floa
     const GnPlan pl = gn_plan(B, S, C, G, sizeof(T));
     const long grid = (long)B * pl.chunks * pl.slices;
     const long gains = dgamma || dbeta ? (C + GN_SUM_C - 1) / GN_SUM_C : 0;
-    if (grid + gains > 0x7fffffff) return MSF2_ERR_ARG;
+    if (!launch_ok(grid + gains, pl.threads)) return MSF2_ERR_ARG;
     float2* part = (float2*)ws;
     float* chan = (float*)((char*)ws + gn_part_bytes(pl, B, sizeof(float2)));
     gn_grad_sums_kernel<T, V, PRE, POST><<<grid, pl.threads, 0, st>>>(dy, x, gamma, beta, stats, lengths, chan, part, pl, S, C, G);

@@ -571,7 +571,7 @@ static int run_recurrence(Rows<const T> x, Rows<const T> gate, const float* h0, 
     float* agg = pl.pieces > 1 ? arena.take<float>((size_t)B * pl.pieces * 2 * C) : nullptr;
     float* kept = pl.pieces > 1 ? arena.take<float>((size_t)B * C) : nullptr;
     const long grid = (long)B * pl.pieces * pl.slices;
-    if (grid > 0x7fffffff) return MSF2_ERR_ARG;
+    if (!launch_ok(grid, 64 * pl.waves)) return MSF2_ERR_ARG;
     return rec_shape<T, false>(pl, C, [&](auto q) {
         typedef decltype(q) Q;
         pl.near = rec_near<Q>(x, C) && rec_near<Q>(gate, C) && rec_near<Q>(h, C);
@@ -592,7 +592,7 @@ static int run_recurrence_backward(Rows<const T> dh, Rows<const T> x, Rows<const
     float* agg = pl.pieces > 1 ? arena.take<float>((size_t)B * pl.pieces * 2 * C) : nullptr;
     float* kept = pl.pieces > 1 ? arena.take<float>((size_t)B * C) : nullptr;
     const long grid = (long)B * pl.pieces * pl.slices;
-    if (grid > 0x7fffffff) return MSF2_ERR_ARG;
+    if (!launch_ok(grid, 64 * pl.waves)) return MSF2_ERR_ARG;
     return rec_shape<T, true>(pl, C, [&](auto q) {
         typedef decltype(q) Q;
         pl.near = rec_near<Q>(dh, C) && rec_near<Q>(x, C) && rec_near<Q>(gate, C) && rec_near<Q>(dx, C) && rec_near<Q>(dgate, C);

@@ -88,6 +88,9 @@ struct Divider {
     __host__ __device__ __forceinline__ unsigned div(unsigned n) const { return (unsigned)((uint64_t)n * m >> shift); }
 };
 
+// Whether a launch of so many workgroups counts its threads in 32 bits, as the hardware does.
+static inline bool launch_ok(long groups, int threads) { return groups * threads < 1l << 32; }
+
 // Frames of utterance b: lengths[b] held to [0, S], all S without lengths.
 __device__ __forceinline__ int frames_of(const int* lengths, int b, int S) {
     return lengths ? min(max(lengths[b], 0), S) : S;

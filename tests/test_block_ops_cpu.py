@@ -184,3 +184,13 @@ def test_overlap_check_agrees_with_the_addresses():
         assert ops._clash(t, u) == bool(at[0] & at[1]), (B, S, C, st, t.storage_offset(), u.storage_offset())
         n += bool(at[0] & at[1])
     assert 500 < n < 2500
+
+
+@pytest.mark.parametrize("call,bad", [
+    *[(call, dict(B=1, S=1, C=C, **kw)) for call, kw in ((_norm, dict(groups=1)), (_norm_backward, dict(groups=1)), (_rec, {}), (_rec_backward, {}), (_drop, {}))
+      for C in (2 ** 30, 2 ** 31 - 8, 2 ** 31 - 1)],
+    (_norm, dict(B=2 ** 24, S=1)), (_norm_backward, dict(B=2 ** 24, S=1, n=1 << 40)), (_norm, dict(B=2 ** 31 - 1, S=1, n=1 << 40)),
+    (_rec, dict(B=2 ** 26, S=1)), (_rec_backward, dict(B=2 ** 26, S=1)), (_rec, dict(B=2 ** 31 - 1, S=1))])
+def test_entry_points_refuse_what_their_indices_do_not_hold(call, bad):
+    """Channels whose index would pass 2^31 within the last lanes, and launches of more threads than the hardware counts."""
+    assert call(_lib.load(), **bad) == -1

@@ -745,3 +745,29 @@ def test_outputs_into_parts_of_frame_major_and_one_frame_tensors():
         assert ops.dropout(x, 0.2, rng, 4, gate, out=gate) is gate and torch.equal(both[..., 40:], drop)
         with pytest.raises(ValueError):
             ops.dropout(x, 0.2, rng, 4, out=both[..., 20:60])
+
+
+def test_the_most_utterances():
+    """As many one-frame utterances as a launch's threads count: the last of them agree with the same rows alone; one more is refused."""
+    B, C, last = (1 << 24) - 1, 2, 1000
+    g = torch.Generator(device=DEV).manual_seed(65)
+    x, dy = (torch.randn(B, 1, C, generator=g, device=DEV) for _ in range(2))
+    y, stats = ops.group_norm_act(x, None, None, 1, eps=0.1, act=1)
+    want = oracle.group_norm(x[-last:].cpu(), None, None, 1, 0.1, 1, False, None, dy[-last:].cpu())
+    close(y[-last:], *want["y"])
+    close(stats[-last:], *want["stats"])
+    close(ops.group_norm_act_backward(dy, x, None, None, stats, 1, act=1)[0][-last:], *want["dx"])
+    B = (1 << 25) - 1
+    x, gate, h0 = (torch.randn(B, 1, 1, generator=g, device=DEV) for _ in range(3))
+    x, gate, h0 = x.to(BF16), gate.to(BF16), h0[:, 0]
+    h, state, saved = ops.gated_recurrence(x, gate, h0, save=True)
+    want = oracle.recurrence(x[-last:].cpu(), gate[-last:].cpu(), h0[-last:].cpu(), None, False, x[-last:].cpu())
+    close(h[-last:], *want["h"])
+    close(state[-last:], *want["last"])
+    for name, v in zip(("dx", "dgate", "dh0"), ops.gated_recurrence_backward(x, x, gate, saved)):
+        close(v[-last:], *want[name], name)
+    with pytest.raises(_lib.Msf2Error):
+        ops.group_norm_act(torch.zeros(1 << 24, 1, C, device=DEV), None, None, 1)
+    x = torch.zeros(1 << 25, 1, 1, dtype=BF16, device=DEV)
+    with pytest.raises(_lib.Msf2Error):
+        ops.gated_recurrence(x, x)
