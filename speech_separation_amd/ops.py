@@ -254,6 +254,7 @@ def _written(*ts):
     for t in ts:
         if t.requires_grad and (t.is_leaf or torch.is_grad_enabled()):
             raise ValueError("a tensor that requires a gradient cannot be written in place here")
+    for t in ts:
         if not t.is_inference():             # those have no version to count
             torch.autograd.graph.increment_version(t)
 
@@ -350,9 +351,9 @@ def gated_recurrence(x, gate, h0=None, lengths=None, reverse=False, last=None, s
         lastp = last.data_ptr()
     else:
         lastp = _aside(last, "last", (B, C), dev)
-        if any(u is not None and _clash(last, u) for u in (x, gate)) or (h0 is not None and _clash(last, h0) and lastp != h0p):
+        if any(_clash(last, u) for u in (x, gate, lengths) if u is not None) or (h0 is not None and _clash(last, h0) and lastp != h0p):
             raise ValueError("last: the output shares memory with another operand")
-        _written(last)
+        _written(last)                       # after all checks: a refused call leaves it as it was
     h = _new(x)
     saved = torch.empty((B, -(-S // _lib.RECURRENCE_SAVE), C), device=dev) if save else None
     if B and S:
@@ -376,18 +377,20 @@ def gated_recurrence_backward(dh, x, gate, saved, dlast=None, lengths=None, reve
     if C < 1:
         raise ValueError("x has no channels")
     dev = x.device
-    if out is None:
-        dx, dgate = _new(x), _new(x)
-        dxr, dgr = (dx.data_ptr(), S * C, C), (dgate.data_ptr(), S * C, C)
-    else:
-        dx, dgate = out
-        dxr = _out_rows(dx, "dx", x, apart=(dh, x, gate, saved, dlast, dgate))
-        dgr = _out_rows(dgate, "dgate", x, apart=(dh, x, gate, saved, dlast))
-        _written(dx, dgate)
     dlp, lp = _aside(dlast, "dlast", (B, C), dev), _aside(lengths, "lengths", (B,), dev, torch.int32)
     savedp = _aside(saved, "saved", (B, -(-S // _lib.RECURRENCE_SAVE), C), dev)
     if savedp is None:
         raise ValueError("saved: expected what gated_recurrence returned with save=True")
+    if out is None:
+        dx, dgate = _new(x), _new(x)
+        dxr, dgr = (dx.data_ptr(), S * C, C), (dgate.data_ptr(), S * C, C)
+    else:
+        if not (isinstance(out, (tuple, list)) and len(out) == 2):
+            raise ValueError("out: expected a pair of tensors")
+        dx, dgate = out
+        dgr = _out_rows(dgate, "dgate", x, apart=(dh, x, gate, saved, dlast, lengths))
+        dxr = _out_rows(dx, "dx", x, apart=(dh, x, gate, saved, dlast, lengths, dgate))
+        _written(dx, dgate)
     if not (B and S):
         return dx, dgate, torch.zeros((B, C), device=dev) if dlast is None else dlast.clone()
     dh0 = torch.empty((B, C), device=dev)
@@ -397,7 +400,7 @@ def gated_recurrence_backward(dh, x, gate, saved, dlast=None, lengths=None, reve
     return dx, dgate, dh0
 
 
-def _dropout(x, p, rng, site, residual, y, yr=None):
+def _dropout(x, p, rng, site, residual, y, given=False):
     xr = _rows(x, "x")
     B, S, C = x.shape
     dev = x.device
@@ -408,11 +411,14 @@ def _dropout(x, p, rng, site, residual, y, yr=None):
     if y.dtype not in _TYPES or (y.dtype != x.dtype and torch.float32 not in (x.dtype, y.dtype)):
         raise ValueError(f"no conversion from {x.dtype} to {y.dtype}")
     rr = (None, 0, 0) if residual is None else _rows(residual, "residual", y)
-    if yr is None:
-        yr = (y.data_ptr(), S * C, C)
     rngp = _aside(rng, "rng", (2,), dev, torch.int64)
     if rngp is None:
         raise ValueError("rng: expected an int64 tensor (seed, step) on the GPU")
+    if given:
+        yr = _out_rows(y, "out", x, same_type=False, apart=(rng,), same=(x, residual))
+        _written(y)
+    else:
+        yr = (y.data_ptr(), S * C, C)
     if B and S and C:
         _call("msf2_dropout", dev, None, (*xr, *rr, *yr, rngp, site, p, B, S, C, _TYPES[x.dtype], _TYPES[y.dtype]))
     return y
@@ -424,13 +430,10 @@ def dropout(x, p, rng, site=0, residual=None, out=None):
     tensor on the GPU, on site, which tells the dropouts of one step apart, and on an element's place, not on strides or
     types (include/msf2.h).  p counts in steps of 2^-16.  Advance rng[1] after a step's backward pass; a captured graph
     draws new masks when the program does.  out: where to write, x or residual themselves if wanted."""
-    if not all(isinstance(t, torch.Tensor) for t in (x, *(() if residual is None else (residual,)))):
-        raise ValueError("x, residual: expected tensors")
+    if not all(isinstance(t, torch.Tensor) for t in (x, *(t for t in (residual, out) if t is not None))):
+        raise ValueError("x, residual, out: expected tensors")
     if out is not None:
-        _rows(x, "x")
-        yr = _out_rows(out, "out", x, same_type=False, apart=(rng,), same=(x, residual))
-        _written(out)
-        return _dropout(x, p, rng, site, residual, out, yr)
+        return _dropout(x, p, rng, site, residual, out, True)
     if residual is not None and residual.shape != x.shape:
         raise ValueError(f"residual: expected shape {tuple(x.shape)}, got {tuple(residual.shape)}")
     return _dropout(x, p, rng, site, residual, _new(x if residual is None else residual))

@@ -771,3 +771,22 @@ def test_the_most_utterances():
     x = torch.zeros(1 << 25, 1, 1, dtype=BF16, device=DEV)
     with pytest.raises(_lib.Msf2Error):
         ops.gated_recurrence(x, x)
+
+
+def test_refused_calls_leave_outputs_unannounced():
+    """A call that is refused has written nothing: autograd still takes the tensors it was to write for unchanged."""
+    x, rng = torch.randn(2, 3, 8, device=DEV), torch.tensor([1, 2], device=DEV)
+    _, last, saved = ops.gated_recurrence(x, x, save=True)
+    a, b = torch.empty_like(x), torch.empty_like(x)
+    long = torch.zeros(2, dtype=torch.int64, device=DEV)
+    calls = [lambda: ops.dropout(x, 2.0, rng, out=a), lambda: ops.dropout(x, 0.1, rng, site=-1, out=a), lambda: ops.dropout(x, 0.1, rng.int(), out=a),
+             lambda: ops.dropout(x, 0.1, 5, out=a), lambda: ops.dropout(x, 0.1, rng, residual=x.double(), out=a), lambda: ops.dropout(x, 0.1, rng, out=3.0),
+             lambda: ops.gated_recurrence_backward(x, x, x, saved[:1], out=(a, b)), lambda: ops.gated_recurrence_backward(x, x, x, 3.0, out=(a, b)),
+             lambda: ops.gated_recurrence_backward(x, x, x, saved, dlast=last[:1], out=(a, b)), lambda: ops.gated_recurrence_backward(x, x, x, saved, dlast=1, out=(a, b)),
+             lambda: ops.gated_recurrence_backward(x, x, x, saved, lengths=long, out=(a, b)), lambda: ops.gated_recurrence_backward(x, x, x, saved, out=(a, None)),
+             lambda: ops.gated_recurrence_backward(x, x, x, saved, out=(a, torch.zeros_like(x, requires_grad=True))),
+             lambda: ops.gated_recurrence_backward(x, x, x, saved, out=a), lambda: ops.gated_recurrence(x, x, lengths=long, last=last)]
+    for f in calls:
+        with pytest.raises(ValueError):
+            f()
+        assert a._version == b._version == last._version == 0
