@@ -35,8 +35,8 @@ class _GroupNormAct(torch.autograd.Function):
 
 class _GatedRecurrence(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, gate, h0, lengths, reverse):
-        h, last, saved = ops.gated_recurrence(x, gate, h0, lengths, reverse, save=any(ctx.needs_input_grad))
+    def forward(ctx, x, gate, h0, lengths, reverse, recording):
+        h, last, saved = ops.gated_recurrence(x, gate, h0, lengths, reverse, save=recording and any(ctx.needs_input_grad))
         ctx.save_for_backward(x, gate, saved, lengths)
         ctx.reverse = reverse
         return h, last
@@ -47,7 +47,7 @@ class _GatedRecurrence(torch.autograd.Function):
         _eager()
         x, gate, saved, lengths = ctx.saved_tensors
         dx, dgate, dh0 = ops.gated_recurrence_backward(_dense(dh), x, gate, saved, dlast.contiguous(), lengths, ctx.reverse)
-        return dx, dgate, dh0 if ctx.needs_input_grad[2] else None, None, None
+        return dx, dgate, dh0 if ctx.needs_input_grad[2] else None, None, None, None
 
 
 class _Dropout(torch.autograd.Function):
@@ -78,7 +78,8 @@ def group_norm_act(x, gamma, beta, groups, eps=1e-5, act=_lib.ACT_NONE, act_firs
 
 def gated_recurrence(x, gate, h0=None, lengths=None, reverse=False):
     """ops.gated_recurrence's (h, last), with gradients of x, gate and h0."""
-    return _GatedRecurrence.apply(x, gate, h0, lengths, reverse)
+    # within apply the gradient mode is always off, and needs_input_grad does not know of it
+    return _GatedRecurrence.apply(x, gate, h0, lengths, reverse, torch.is_grad_enabled())
 
 
 def dropout(x, p, rng, site=0, residual=None):

@@ -194,3 +194,22 @@ def test_overlap_check_agrees_with_the_addresses():
 def test_entry_points_refuse_what_their_indices_do_not_hold(call, bad):
     """Channels whose index would pass 2^31 within the last lanes, and launches of more threads than the hardware counts."""
     assert call(_lib.load(), **bad) == -1
+
+
+def test_autograd_keeps_states_for_a_backward_pass_only(monkeypatch):
+    """With a learned first state, say: its gradient is asked for, but not under no_grad or inference_mode."""
+    from speech_separation_amd import autograd
+    asked = []
+
+    def fake(x, gate, h0, lengths, reverse, save):
+        asked.append(save)
+        return x * 1, h0 * 1, torch.zeros(1) if save else None
+
+    monkeypatch.setattr(ops, "gated_recurrence", fake)
+    x, h0 = torch.zeros(2, 3, 8), torch.zeros(2, 8, requires_grad=True)
+    for mode, want in ((torch.enable_grad, True), (torch.no_grad, False), (torch.inference_mode, False)):
+        with mode():
+            autograd.gated_recurrence(x, x, h0)
+        assert asked.pop() is want, mode
+    autograd.gated_recurrence(x, x, h0.detach())
+    assert asked.pop() is False
