@@ -545,7 +545,8 @@ template <class T, int V, int LC, int R, class F> static int rec_waves(const Rec
 }
 template <class T, int VEC, class F> static int rec_lanes(const RecPlan& pl, F f) {
     constexpr int LC = 256 / (VEC * sizeof(T)), R = REC_VALUES / VEC;
-    if (pl.vec == 1) return rec_waves<T, 1, LC / 2, R>(pl, f);
+    if constexpr (VEC * sizeof(T) == 8)      // 4-byte accesses are for even widths, which are never narrower
+        if (pl.vec == 1) return rec_waves<T, 1, LC / 2, R>(pl, f);
     return pl.lanes == LC ? rec_waves<T, VEC, LC, R>(pl, f) : rec_waves<T, VEC, LC / 2, R>(pl, f);
 }
 template <class T, bool BACK, class F> static int rec_shape(const RecPlan& pl, int C, F f) {
