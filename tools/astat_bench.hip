@@ -1,5 +1,5 @@
 // Diagnostic: the register-resident-activation bf16 projection kernel alone, on random data, timed with HIP events.
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -Ispeech_separation_amd/csrc -Wno-inline-asm -o tools/astat_bench tools/astat_bench.hip [-DMSF2_DIAG_...]
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -Ispeech_separation_amd/csrc -Wno-inline-asm -o tools/astat_bench tools/astat_bench.hip [-DMSF2_DIAG_...]
 //   tools/astat_bench [batch [N]]
 #include "msf2_common.h"
 #include "msf2_gemm.h"

@@ -2,7 +2,7 @@
 // two-product kernel (per k tile: a piece of 128 activation rows of this workgroup's row tile + a piece of 128 weight
 // rows shared by every workgroup), without MFMAs, LDS reads or an epilogue.  Varies the bytes per row piece
 // (64 / 128 / 256), the ring depth, workgroups per CU and the source (activations only / weights only / both).
-//   hipcc --offload-arch=gfx950 -O3 -o /tmp/lds_copy_rate tools/lds_copy_rate.hip && /tmp/lds_copy_rate
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -o /tmp/lds_copy_rate tools/lds_copy_rate.hip && /tmp/lds_copy_rate
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

@@ -1,5 +1,5 @@
 // Diagnostic: the bf16 key/value-summary kernel alone, on random data, timed with HIP events.
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -Ispeech_separation_amd/csrc -Iinclude -Wno-inline-asm -o tools/linkv_bench tools/linkv_bench.hip [-DMSF2_DIAG_LKV_...]
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -Ispeech_separation_amd/csrc -Iinclude -Wno-inline-asm -o tools/linkv_bench tools/linkv_bench.hip [-DMSF2_DIAG_LKV_...]
 //   tools/linkv_bench [batch]
 #include "msf2_common.h"
 #include "msf2_gemm.h"

@@ -2,7 +2,7 @@
 // busy, random operands, 2 blocks of 4 waves per CU), as the ingredients of a real GEMM
 // main loop are added one at a time: LDS fragment reads, a barrier per 64 MFMAs,
 // LDS writes, global loads.
-// build: hipcc -O3 --offload-arch=gfx950 tools/mfma_peak.hip -o tools/mfma_peak
+// build: hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/mfma_peak.hip -o tools/mfma_peak
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

@@ -1,5 +1,5 @@
 // Diagnostic: the register-resident two-product TCN contraction alone against a host evaluation of sampled outputs.
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -Ispeech_separation_amd/csrc -Iinclude -Wno-inline-asm -o tools/tcn_astat_check tools/tcn_astat_check.hip
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -Ispeech_separation_amd/csrc -Iinclude -Wno-inline-asm -o tools/tcn_astat_check tools/tcn_astat_check.hip
 #include "msf2_common.h"
 #include "msf2_gemm.h"
 #include "msf2_gemm_bf16.h"
