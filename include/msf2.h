@@ -336,7 +336,9 @@ int msf2_pit_si_snr_noalloc(const float* est, const float* src, float* si_snr, f
  * Activations are [B, S, C] in one of the element types below.  Channels are contiguous; `*_batch` and `*_row` are the
  * strides of the batch and of a frame in ELEMENTS, so a tensor may be a slice of a wider one (value and gate side by side
  * as one projection writes them).  No alignment beyond the element's is asked for.  Arithmetic, statistics, states and
- * sums are fp32 or wider whatever the element type.  Outputs must not overlap inputs, except where stated.
+ * sums are fp32 or wider whatever the element type.  Sigmoids (of SiLU and of the gates) are good to a few roundings of 2^-24 with
+ * fp32 operands; with 16-bit ones the smaller of sigmoid(v) and 1 - sigmoid(v) has a relative error of |v| 2^-24 more, and so have the
+ * fp32 results that come of it.  Outputs must not overlap inputs, except where stated.
  * `lengths` (int32 [B] on the device, or null: all S): frames at and past lengths[b] belong to no utterance.  They are not
  * read into any result, whatever they hold, and outputs are zero there.  Values outside [0, S] count as the nearer end.
  * S and C are below 2^30 and B S C is at most 2^46; a call whose launch would take 2^32 threads or more (from 2^24 utterances of a frame
@@ -370,6 +372,8 @@ size_t msf2_group_norm_act_backward_ws_bytes(int B, int S, int C, int groups, in
  *   last  fp32 [B][C], may be null or h0 itself: the state after the last frame walked (h0 for an empty utterance).
  *   saved fp32 [B][ceil(S / MSF2_RECURRENCE_SAVE)][C], null unless the backward pass follows: the state before every
  *         MSF2_RECURRENCE_SAVE-th frame walked, from which the backward pass computes h again.
+ * Frames are joined in runs, each as (product of its gates, what it adds), so a state that has become infinite may be NaN some
+ * frames later, where a walk frame by frame would leave it infinite; finite states and other channels are not touched by that.
  * Backward: dh, and dlast (fp32 [B][C], null: zeros), the gradient of `last`, give dx, dgate and dh0 (fp32 [B][C], may be null
  * or dlast itself). */
 #define MSF2_RECURRENCE_SAVE 32

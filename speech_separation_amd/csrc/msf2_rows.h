@@ -97,7 +97,8 @@ __device__ __forceinline__ int frames_of(const int* lengths, int b, int S) {
 }
 
 // p = 1 / (1 + t) and q = 1 - p = t p, t = e^-v: neither cancels.  A rounding d of v log2 e is a relative error d ln 2 of t, which p takes
-// q times and q takes p times: FINE (fp32 operands) adds the part that the product's rounding left out.  Values beyond 87 are
+// q times and q takes p times: FINE (fp32 operands) adds the part that the product's rounding left out.  Without it the smaller of
+// p and q is off by up to |v| 2^-24 of itself, 2^-18 at the most: far below the steps of the 16-bit operands that v comes from.  Values beyond 87 are
 // held there (e^87 and its inverse are normal numbers; maximum and minimum keep NaN).
 template <bool FINE> __device__ __forceinline__ void sigmoid_pair(float v, float& p, float& q) {
     constexpr float LOG2E = 1.44269504088896f, LN2 = 0.693147180559945f;
@@ -111,7 +112,7 @@ template <bool FINE> __device__ __forceinline__ void sigmoid_pair(float v, float
 }
 template <class T> constexpr bool fine() { return sizeof(T) == 4; }
 
-// v p of minus infinity is 0, not a product of infinity and the least p
+// v p of v far below zero ends at -87 e^-87, -1e-36, where v itself would give a product of infinity and the least p
 __device__ __forceinline__ float silu_of(float v, float p) { return __builtin_elementwise_maximum(v, -87.f) * p; }
 
 template <int ACT, bool FINE> __device__ __forceinline__ float act_f(float v) {
